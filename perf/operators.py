@@ -43,21 +43,21 @@ def listed():
         # a handful of requests decoding together, skewed expert load
         _moe("moe 5 tokens", 5, 2048, 512, 256, 8, True, bias=True),
         # sixteen tokens of a small model without a shared expert
-        _moe("moe 16 tokens, 64 experts", 16, 1024, 256, 64, 4, False),
+        _moe("moe 16 tokens 64 experts", 16, 1024, 256, 64, 4, False),
         # the largest batch of the path: most experts are touched
-        _moe("moe 16 tokens, 256 experts", 16, 2048, 512, 256, 8, True, norm=True, residual=True),
+        _moe("moe 16 tokens 256 experts", 16, 2048, 512, 256, 8, True, norm=True, residual=True),
         # one request's adapter beside a square projection
         _lora("lora 1 token", 1, 2048, 2048, "q8_0", 16, 4, "f16"),
         # sixteen requests, eight adapters of rank up to 64, a wide 4-bit projection
-        _lora("lora 16 tokens, 4 bits", 16, 4096, 12288, "q4_0", 64, 8, "bf16"),
+        _lora("lora 16 tokens 4 bits", 16, 4096, 12288, "q4_0", 64, 8, "bf16"),
         # an odd batch and odd sizes, adapters kept in 32 bits
-        _lora("lora 37 tokens, ragged", 37, 1024, 3001, "q4_0", 12, 5, "f32"),
+        _lora("lora 37 tokens ragged", 37, 1024, 3001, "q4_0", 12, 5, "f32"),
         # the LM head of a decode batch with sixteen adapters
-        _lora("lora 64 tokens, LM head", 64, 2048, 151936, "q8_0", 16, 16, "f16"),
+        _lora("lora 64 tokens LM head", 64, 2048, 151936, "q8_0", 16, 16, "f16"),
         # the sampled token of one request with its twenty best alternatives
         _logprobs("logprobs 1 row", 1, 151936, "f32", 20, 1),
         # a masked vocabulary, several candidate tokens a row, rows at an odd stride
-        _logprobs("logprobs 7 rows, masked", 7, 50257, "f16", 20, 4, masked=True, pad=3),
+        _logprobs("logprobs 7 rows masked", 7, 50257, "f16", 20, 4, masked=True, pad=3),
         # a decode batch
         _logprobs("logprobs 64 rows", 64, 151936, "f32", 5, 1),
         # scoring a prompt
