@@ -48,6 +48,7 @@ extern "C" {
 #define PI_QT_F16 1
 #define PI_QT_Q4_0 2
 #define PI_QT_Q8_0 8
+#define PI_QT_BF16 30
 
 /* pi_moe_forward flags */
 #define PI_FWD_RMSNORM 1  /* apply RMSNorm (unit weight) before routing: model/mod.rs:1239 */
@@ -320,6 +321,25 @@ int pi_sparse_ffn_forward(pi_ctx* ctx, pi_sparse_ffn* ffn, const float* x, int64
  * for T inputs a [T][n_in]; W1 [n_hidden][n_in], W2 [n_out][n_hidden] row-major f32. */
 int pi_predictor_forward(pi_ctx* ctx, const float* a, int64_t T, const float* W1, const float* b1, const float* W2,
                          const float* b2, int64_t n_in, int64_t n_hidden, int64_t n_out, float* probs, void* stream);
+
+/* ---- scores of tokens from logits ---------------------------------------
+ * No reference counterpart (its quality benchmark compares logit vectors on the
+ * host, src/benchmark/mod.rs:45-240). For each of T rows of V logits (row t starts
+ * at logits + t * ld elements; dtype PI_QT_F32, PI_QT_F16 or PI_QT_BF16, any
+ * alignment of that type), in one pass, with every sum in f32:
+ *   logp    [T][n_targets]  log softmax at targets[t][j] (int64); 0 for a negative
+ *                           target (padding); a target >= V gives NaN and a device
+ *                           error (pi_ctx_check -> PI_ERR_INDEX)
+ *   entropy [T]             -sum p log p (natural logarithm); may be NULL
+ *   top_ids, top_logp [T][n_top]  the n_top <= 32 most likely tokens, descending, ties
+ *                           to the lowest index; -1 and -inf where fewer have p > 0
+ * A logit of -inf is a masked token (p = 0, logp -inf, never an alternative). A row
+ * with nothing else has entropy 0, logp -inf and ids -1; a row that holds a NaN or
+ * +inf has no distribution: its values are NaN and its ids -1.
+ * Needs no scratch: calls on any streams and captured graphs are independent. */
+int pi_token_logprobs(pi_ctx* ctx, const void* logits, int32_t dtype, int64_t T, int64_t V, int64_t ld,
+                      const int64_t* targets, int64_t n_targets, int32_t n_top, float* logp, float* entropy,
+                      int32_t* top_ids, float* top_logp, void* stream);
 
 /* ---- synthetic inputs (benchmarks and tests; no reference counterpart) --
  * out[i] = std * N(0,1) from SplitMix64 (model/mod.rs:2041-2061) + Box-Muller,

@@ -13,7 +13,7 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libpi_moe.so"
 
 PI_OK, PI_ERR_ARG, PI_ERR_INDEX, PI_ERR_SHORT, PI_ERR_OOM, PI_ERR_CUDA, PI_ERR_TIMEOUT = range(7)
-PI_QT_F32, PI_QT_F16, PI_QT_Q4_0, PI_QT_Q8_0 = 0, 1, 2, 8
+PI_QT_F32, PI_QT_F16, PI_QT_Q4_0, PI_QT_Q8_0, PI_QT_BF16 = 0, 1, 2, 8, 30
 PI_EP_MAX_WORLD, PI_EP_HANDLE_BYTES = 64, 64
 PI_FWD_RMSNORM, PI_FWD_RESIDUAL, PI_FWD_FORCE_GEMV, PI_FWD_FORCE_GEMM, PI_FWD_FAST_SUM = 1, 2, 4, 8, 16
 
@@ -82,6 +82,7 @@ SIGNATURES = {
     "pi_predictor_forward": (_INT, [_P, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _P, _P]),
     "pi_hot_lists_from_probs": (_INT, [_P, _P, _I64, _I64, C.c_float, _I64, _I64, _P, _P, _P]),
     "pi_hot_lists_broadcast": (_INT, [_P, _P, _I64, _I64, _P, _P, _P]),
+    "pi_token_logprobs": (_INT, [_P, _P, _I32, _I64, _I64, _I64, _P, _I64, _I32, _P, _P, _P, _P, _P]),
     "pi_synth_normal": (_INT, [_P, C.c_uint64, C.c_uint64, _I64, C.c_float, _P, _P]),
     "pi_synth_normal_host": (_INT, [C.c_uint64, C.c_uint64, _I64, C.c_float, _P]),
 }
@@ -131,6 +132,17 @@ class Context:
             ctx = cls(device)
             with _lock:
                 cls._default[device] = ctx
+        return ctx
+
+    @classmethod
+    def of(cls, device: int) -> "Context":
+        """The default context of ``device``, leaving the current device as it is."""
+        ctx = cls._default.get(device)
+        if ctx is None:
+            import torch
+
+            with torch.cuda.device(device):
+                ctx = cls.default(device)
         return ctx
 
     def check(self, rc: int) -> None:

@@ -7,7 +7,7 @@
 #define PI_DEV __device__ __forceinline__
 
 // GGML type ids used at the C ABI (same numbering as ggml_type).
-enum { PI_QT_F32 = 0, PI_QT_F16 = 1, PI_QT_Q4_0 = 2, PI_QT_Q8_0 = 8 };
+enum { PI_QT_F32 = 0, PI_QT_F16 = 1, PI_QT_Q4_0 = 2, PI_QT_Q8_0 = 8, PI_QT_BF16 = 30 };
 
 // Device error word bits (written by kernels, read by pi_ctx_check).
 enum { PI_DEVERR_INDEX = 1, PI_DEVERR_TIMEOUT = 2, PI_DEVERR_SHAPE = 4 };

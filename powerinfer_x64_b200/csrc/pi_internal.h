@@ -137,6 +137,19 @@ struct PiProfScope {
     ~PiProfScope();
 };
 int pi_cuda_check(pi_ctx* ctx, cudaError_t e, const char* what);
+// Makes `device` current for a scope and the previous device current again after it.
+struct PiDeviceGuard {
+    int prev = -1;
+    explicit PiDeviceGuard(int device) {
+        int cur = -1;
+        if (cudaGetDevice(&cur) == cudaSuccess && cur != device && cudaSetDevice(device) == cudaSuccess) prev = cur;
+    }
+    ~PiDeviceGuard() {
+        if (prev >= 0) cudaSetDevice(prev);
+    }
+    PiDeviceGuard(const PiDeviceGuard&) = delete;
+    PiDeviceGuard& operator=(const PiDeviceGuard&) = delete;
+};
 // Raises fn's dynamic shared-memory limit to `bytes` on the current device (once per
 // kernel and device; no-op at or below the 48 KB default).
 void pi_smem_attr(const void* fn, size_t bytes);

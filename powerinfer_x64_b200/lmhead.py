@@ -17,6 +17,7 @@ import numpy as np
 
 from . import quant
 from ._lib import Context, lib, ptr, stream_ptr
+from .logprobs import token_logprobs
 
 
 def lm_head_slices(n_out: int, n_gpus: int):
@@ -85,6 +86,11 @@ class LmHead:
         if self.world == 1:
             return local
         return gather_slices(local, self.slices, self.group)
+
+    def logprobs(self, x, targets=None, n_top: int = 0):
+        """``token_logprobs`` of the full logits of x [T, n_in]: log probabilities of the
+        given tokens, entropy and the n_top best alternatives."""
+        return token_logprobs(self.forward(x), targets=targets, n_top=n_top)
 
 
 def gather_slices(local, slices, group=None):
