@@ -208,8 +208,10 @@ int pi_prefill_experts(pi_ctx* ctx, const pi_moe_layer* L, const ExpertArgs& a, 
                        const __half* xth, const __half* xtl, int64_t T, __half* hh, __half* hl, cudaStream_t st);
 // Builds L->maps (layer create; no-op for layers the GEMM does not take).
 int pi_prefill_prepare(pi_ctx* ctx, pi_moe_layer* L);
-// n_embd and expert width the prefill GEMM tiles (whole 512-row / 128-row CTA blocks)
-inline bool pi_prefill_shape_ok(int64_t d, int64_t f) { return d % 512 == 0 && f % 128 == 0; }
+// n_embd and expert width the prefill GEMM tiles: whole 512-row / 128-row CTA blocks, and
+// f16 block scales of a down row (f / 32 of them) that fill whole 16-byte units, as the
+// stride of a tensor map must
+inline bool pi_prefill_shape_ok(int64_t d, int64_t f) { return d % 512 == 0 && f % 256 == 0; }
 constexpr int PI_GEMM_NT = 256;     // slots per prefill work item (Q4_0)
 constexpr int PI_GEMM_NT_Q8 = 128;  // slots per prefill work item (Q8_0)
 // Exact Q8_0 prefill expert products (pi_prefill_q8.cu): gate/up + SwiGLU + Q8_0 h

@@ -517,7 +517,7 @@ int pi_prefill_experts(pi_ctx* ctx, const pi_moe_layer* L, const ExpertArgs& a, 
     static_assert(MT * DN_MPC == 512 && MT * GU_MPC == 128, "pi_prefill_shape_ok matches the CTA blocks");
     if (!pi_prefill_shape_ok(a.d, a.f) || (L->has_shared && L->f_sh != L->f))
         return pi_set_error(ctx, PI_ERR_ARG,
-                            "prefill GEMM: n_embd must be a multiple of 512, expert widths equal and a multiple of 128");
+                            "prefill GEMM: n_embd must be a multiple of 512, expert widths equal and a multiple of 256");
     if (!L->maps_ok) return pi_set_error(ctx, PI_ERR_CUDA, "prefill GEMM: weight tensor maps unavailable");
     CUtensorMap mhh, mhl;
     if (!act_map(&mhh, hh, n_slots, a.f) || !act_map(&mhl, hl, n_slots, a.f))
