@@ -65,6 +65,7 @@ typedef struct pi_ctx pi_ctx;
 typedef struct pi_moe_layer pi_moe_layer;
 typedef struct pi_sparse_ffn pi_sparse_ffn;
 typedef struct pi_ep_comm pi_ep_comm;
+typedef struct pi_proj pi_proj;
 
 #define PI_EP_MAX_WORLD 64    /* ranks of one expert-parallel group          */
 #define PI_EP_HANDLE_BYTES 64 /* bytes of one rank's exported memory handle  */
@@ -321,6 +322,45 @@ int pi_sparse_ffn_forward(pi_ctx* ctx, pi_sparse_ffn* ffn, const float* x, int64
  * for T inputs a [T][n_in]; W1 [n_hidden][n_in], W2 [n_out][n_hidden] row-major f32. */
 int pi_predictor_forward(pi_ctx* ctx, const float* a, int64_t T, const float* W1, const float* b1, const float* W2,
                          const float* b2, int64_t n_in, int64_t n_hidden, int64_t n_out, float* probs, void* stream);
+
+/* ---- a shared projection beside the requests' low-rank adapters ---------
+ * No reference counterpart: the reference projects one token per call
+ * (quant::matvec_col_major, src/quant/mod.rs:939-970; the LM head of
+ * src/cuda/mod.rs:462-537) and has no adapters. Weights W [ne0 = n_in, ne1 = n_out]
+ * in GGUF Q8_0 or Q4_0 blocks (reference nibble order) are laid out once;
+ * raw_len < the shape's bytes -> PI_ERR_SHORT. n_in % 32 == 0. */
+int pi_proj_create(pi_ctx* ctx, const void* raw, uint64_t raw_len, int32_t qtype, int64_t n_in, int64_t n_out,
+                   int32_t src_on_host, pi_proj** out);
+void pi_proj_destroy(pi_proj* proj);
+
+/* Adapters of the requests, caller-owned device memory, read at every call (so an
+ * adapter may be replaced between calls): adapter i adds
+ * scales[i] * b[i][:, :ranks[i]] (a[i][:ranks[i], :] x). */
+typedef struct pi_lora_bank {
+    const void* a;         /* [n_adapters][max_rank][n_in], 16-byte aligned            */
+    const void* b;         /* [n_adapters][n_out][max_rank], 16-byte aligned           */
+    const int32_t* ranks;  /* [n_adapters], 0..max_rank; NULL: max_rank. What a and b
+                              hold past an adapter's rank is not used                  */
+    const float* scales;   /* [n_adapters]; NULL: 1                                    */
+    int32_t dtype;         /* of a and b: PI_QT_F32, PI_QT_F16 or PI_QT_BF16           */
+    int32_t n_adapters;
+    int64_t max_rank;      /* a multiple of 8, at most 1024                            */
+} pi_lora_bank;
+
+/* y [T][n_out] = W x_t + the adapter of token t, for x [T][n_in] f32 (16-byte
+ * aligned). adapter_ids [T] int32: the token's adapter, a negative id for none; an id
+ * >= n_adapters is a device error (pi_ctx_check -> PI_ERR_INDEX) and adds nothing.
+ * bank and adapter_ids NULL: the projection alone.
+ * Q8_0 weights quantise x to Q8_0 as pi_matvec_col_major does; a block then adds its
+ * exact integer dot times d_w d_x with one fused multiply-add, so results equal
+ * pi_matvec_col_major's to f32 rounding, not bit for bit. Q4_0 weights use f32 x (in
+ * two f16 terms, within 2^-22 of each value); a token with a NaN or infinity gives NaN.
+ * workspace: pi_proj_workspace(proj, T, bank) bytes, 256-byte aligned, that nothing
+ * else uses until the call's work is done (two captured graphs need one each). NULL:
+ * the stream's scratch arena (pi_ctx_reserve before a capture). */
+uint64_t pi_proj_workspace(const pi_proj* proj, int64_t T, const pi_lora_bank* bank);
+int pi_proj_forward(pi_ctx* ctx, const pi_proj* proj, const float* x, int64_t T, const pi_lora_bank* bank,
+                    const int32_t* adapter_ids, float* y, void* workspace, uint64_t workspace_bytes, void* stream);
 
 /* ---- scores of tokens from logits ---------------------------------------
  * No reference counterpart (its quality benchmark compares logit vectors on the

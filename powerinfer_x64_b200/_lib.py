@@ -42,6 +42,11 @@ class PiMoeLayerDesc(C.Structure):
     ]
 
 
+class PiLoraBank(C.Structure):
+    _fields_ = [("a", _P), ("b", _P), ("ranks", _P), ("scales", _P), ("dtype", _I32), ("n_adapters", _I32),
+                ("max_rank", _I64)]
+
+
 # name -> (restype, argtypes); every symbol include/pi_moe.h declares.
 SIGNATURES = {
     "pi_ctx_create": (_INT, [_INT, C.POINTER(_P)]),
@@ -82,6 +87,10 @@ SIGNATURES = {
     "pi_predictor_forward": (_INT, [_P, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _P, _P]),
     "pi_hot_lists_from_probs": (_INT, [_P, _P, _I64, _I64, C.c_float, _I64, _I64, _P, _P, _P]),
     "pi_hot_lists_broadcast": (_INT, [_P, _P, _I64, _I64, _P, _P, _P]),
+    "pi_proj_create": (_INT, [_P, _P, C.c_uint64, _I32, _I64, _I64, _I32, C.POINTER(_P)]),
+    "pi_proj_destroy": (None, [_P]),
+    "pi_proj_workspace": (C.c_uint64, [_P, _I64, C.POINTER(PiLoraBank)]),
+    "pi_proj_forward": (_INT, [_P, _P, _P, _I64, C.POINTER(PiLoraBank), _P, _P, _P, C.c_uint64, _P]),
     "pi_token_logprobs": (_INT, [_P, _P, _I32, _I64, _I64, _I64, _P, _I64, _I32, _P, _P, _P, _P, _P]),
     "pi_synth_normal": (_INT, [_P, C.c_uint64, C.c_uint64, _I64, C.c_float, _P, _P]),
     "pi_synth_normal_host": (_INT, [C.c_uint64, C.c_uint64, _I64, C.c_float, _P]),
