@@ -28,7 +28,7 @@ namespace {
 
 constexpr int LP_NT = 256;       // threads of a CTA
 constexpr int LP_W = LP_NT / 32;
-constexpr int LP_U = 4;          // 16-byte loads a thread keeps in flight
+constexpr int LP_U = 2;          // 16-byte loads of a step; the next step's are in flight
 constexpr int LP_MAXC = 16;      // CTAs of a cluster at most
 constexpr int LP_MAXTOP = 32;    // alternatives at most
 constexpr float LP_LOG2E = 1.4426950408889634f;
@@ -51,12 +51,6 @@ struct LpStat {
     float m, s, w;
 };
 
-// max that gives NaN when an operand is NaN (fmaxf drops it)
-PI_DEV float max_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
 PI_DEV float ex2(float a) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a));
@@ -73,6 +67,16 @@ PI_DEV void lp_join(LpStat& a, const LpStat& b) {
     a.w = fmaf(da, a.s, a.w) * ea + fmaf(db, b.s, b.w) * eb;
     a.s = a.s * ea + b.s * eb;
     a.m = m;
+}
+
+template <int N>
+PI_DEV float lp_max(const float* f) {
+    float a = fmaxf(f[0], f[1]), b = fmaxf(f[2], f[3]);
+    if constexpr (N == 8) {
+        a = fmaxf(a, fmaxf(f[4], f[5]));
+        b = fmaxf(b, fmaxf(f[6], f[7]));
+    }
+    return fmaxf(a, b);
 }
 
 // One 64-bit key per value: larger for a larger logit and, where they tie (-0 and 0 too),
@@ -172,24 +176,38 @@ struct LpTop {
     }
 };
 
-// The n best of `cnt` distinct keys in `all` to best[0..n) (0 where there are fewer):
-// a key's place is the number of larger ones.
+// The n best of `cnt` distinct keys in `all` to best[0..n) (0 where there are fewer): a
+// key's place is the number of larger ones, counted by four lanes.
 PI_DEV void lp_rank(const uint64_t* all, int cnt, uint64_t* best, int n, int tid) {
     if (tid < n && tid >= cnt) best[tid] = 0;
-    for (int i = tid; i < cnt; i += LP_NT) {
-        const uint64_t k = all[i];
+    for (int i0 = 0; i0 < cnt; i0 += LP_NT / 4) {
+        const int i = i0 + (tid >> 2);
+        const uint64_t k = i < cnt ? all[i] : ~0ull;
         int r = 0;
-        for (int j = 0; j < cnt; ++j) r += all[j] > k;
-        if (r < n) best[r] = k;
+        for (int j = tid & 3; j < cnt; j += 4) r += all[j] > k;
+        r += __shfl_xor_sync(0xffffffffu, r, 1);
+        r += __shfl_xor_sync(0xffffffffu, r, 2);
+        if (i < cnt && r < n && (tid & 3) == 0) best[r] = k;
+    }
+}
+
+// Joins the states of the lanes whose numbers differ below `width`, a power of two.
+PI_DEV void lp_join_lanes(LpStat& st, int width) {
+    for (int o = width >> 1; o > 0; o >>= 1) {
+        LpStat b;
+        b.m = __shfl_xor_sync(0xffffffffu, st.m, o);
+        b.s = __shfl_xor_sync(0xffffffffu, st.s, o);
+        b.w = __shfl_xor_sync(0xffffffffu, st.w, o);
+        lp_join(st, b);
     }
 }
 
 // Row blockIdx.x / C, share blockIdx.x % C. The first LP_U loads of a thread give, over
 // groups of four lanes, 64 maxima: the n-th largest of them is reached by n values at
 // least, so only what reaches it is kept from the start (about n values of the first
-// 4096 or 8192, then n / i of the i-th load), and the buffers hardly ever fill.
+// 2048 or 4096, then n / i of the i-th step), and the buffers hardly ever fill.
 template <typename ET, bool TOP>
-__global__ __launch_bounds__(LP_NT) void k_token_logprobs(const LogprobArgs a) {
+__global__ __launch_bounds__(LP_NT, 3) void k_token_logprobs(const LogprobArgs a) {
     constexpr int NV = 16 / (int)sizeof(ET);
     constexpr int CAP = 64 + 32 * NV;  // n kept after compact() and one load of every lane
     __shared__ uint64_t s_buf[TOP ? LP_W * CAP : 1];
@@ -234,12 +252,19 @@ __global__ __launch_bounds__(LP_NT) void k_token_logprobs(const LogprobArgs a) {
         if (lane < head) scalar(v);
         if constexpr (TOP) top.template add<1>(&v, v, (uint32_t)lane);
     }
-    bool first = true;
-    for (int64_t v0 = (int64_t)rank * LP_NT + tid; v0 - tid < nvec || first; v0 += LP_U * step) {
-        int4 q[LP_U];
+    // the next LP_U loads are on their way while the current ones are worked on
+    int4 q[LP_U], qn[LP_U];
+    int64_t v0 = (int64_t)rank * LP_NT + tid;
 #pragma unroll
-        for (int u = 0; u < LP_U; ++u)
-            if (v0 + u * step < nvec) q[u] = ld_stream(xv + v0 + u * step);
+    for (int u = 0; u < LP_U; ++u)
+        if (v0 + u * step < nvec) qn[u] = ld_stream(xv + v0 + u * step);
+    bool first = true;
+    for (; v0 - tid < nvec || first; v0 += LP_U * step) {
+#pragma unroll
+        for (int u = 0; u < LP_U; ++u) {
+            q[u] = qn[u];
+            if (v0 + (LP_U + u) * step < nvec) qn[u] = ld_stream(xv + v0 + (LP_U + u) * step);
+        }
         if constexpr (TOP) {
             if (first) {
                 float mx = -INFINITY;
@@ -248,17 +273,23 @@ __global__ __launch_bounds__(LP_NT) void k_token_logprobs(const LogprobArgs a) {
                     if (v0 + u * step < nvec) {
                         float f[NV];
                         lp_unpack<ET>(q[u], f);
-#pragma unroll
-                        for (int j = 0; j < NV; ++j) mx = fmaxf(mx, f[j]);
+                        mx = fmaxf(mx, lp_max<NV>(f));
                     }
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
                 if ((lane & 3) == 0) s_max[tid >> 2] = mx;
                 __syncthreads();
-                if (tid < 64) {
-                    const float mine = s_max[tid];
+                {
+                    const int i = tid >> 2;  // four lanes count the maxima above the i-th
+                    const float mine = s_max[i];
                     int r = 0;
-                    for (int j = 0; j < 64; ++j) r += s_max[j] > mine || (s_max[j] == mine && j < tid);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const int o = (tid & 3) + 4 * j;
+                        r += s_max[o] > mine || (s_max[o] == mine && o < i);
+                    }
+                    r += __shfl_xor_sync(0xffffffffu, r, 1);
+                    r += __shfl_xor_sync(0xffffffffu, r, 2);
                     if (r == a.n_top - 1) s_thr = mine;
                 }
                 __syncthreads();
@@ -273,20 +304,29 @@ __global__ __launch_bounds__(LP_NT) void k_token_logprobs(const LogprobArgs a) {
             float vmax = -INFINITY;
             if (live) {
                 lp_unpack<ET>(q[u], f);
-#pragma unroll
-                for (int j = 0; j < NV; ++j) vmax = fmaxf(vmax, f[j]);
+                vmax = lp_max<NV>(f);
                 if (vmax > st.m) {
                     const float dm = lp_shift(st.m, vmax), e = ex2(dm * LP_LOG2E);
                     st.w = fmaf(dm, st.s, st.w) * e;
                     st.s *= e;
                     st.m = vmax;
                 }
+                const uint64_t m2 = pack2(-st.m, -st.m), l2 = pack2(LP_LOG2E, LP_LOG2E);
+                uint64_t s2 = 0, w2 = 0;
 #pragma unroll
-                for (int j = 0; j < NV; ++j) {
-                    const float t = lp_shift(f[j], st.m), e = ex2(t * LP_LOG2E);
-                    st.s += e;
-                    st.w = fmaf(t, e, st.w);
+                for (int j = 0; j < NV; j += 2) {
+                    float2 t = unpack2(add2(pack2(f[j], f[j + 1]), m2));
+                    t.x = max_nan(t.x, -200.0f);
+                    t.y = max_nan(t.y, -200.0f);
+                    const uint64_t tt = pack2(t.x, t.y);
+                    const float2 g = unpack2(mul2(tt, l2));
+                    const uint64_t e = pack2(ex2(g.x), ex2(g.y));
+                    s2 = add2(s2, e);
+                    w2 = fma2(tt, e, w2);
                 }
+                const float2 sp = unpack2(s2), wp = unpack2(w2);
+                st.s += sp.x + sp.y;
+                st.w += wp.x + wp.y;
             } else {
 #pragma unroll
                 for (int j = 0; j < NV; ++j) f[j] = -INFINITY;
@@ -304,14 +344,7 @@ __global__ __launch_bounds__(LP_NT) void k_token_logprobs(const LogprobArgs a) {
     }
 
     // join: lanes, warps, then the CTAs of the cluster
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        LpStat b;
-        b.m = __shfl_xor_sync(0xffffffffu, st.m, o);
-        b.s = __shfl_xor_sync(0xffffffffu, st.s, o);
-        b.w = __shfl_xor_sync(0xffffffffu, st.w, o);
-        lp_join(st, b);
-    }
+    lp_join_lanes(st, 32);
     if (lane == 0) s_stat[warp] = st;
     if constexpr (TOP) {
         if (lane == 0) s_cnt[warp] = top.cnt;
@@ -333,42 +366,47 @@ __global__ __launch_bounds__(LP_NT) void k_token_logprobs(const LogprobArgs a) {
         for (int i = lane; i < top.cnt; i += 32) s_all[at + i] = top.buf[i];
         __syncthreads();
         lp_rank(s_all, total, s_best, a.n_top, tid);
+    } else {
+        __syncthreads();
     }
-    __syncthreads();
-    if (tid == 0) {
-        LpStat t = s_stat[0];
-        for (int i = 1; i < LP_W; ++i) lp_join(t, s_stat[i]);
-        s_cta = t;
+    if (warp == 0) {
+        LpStat t = s_stat[lane % LP_W];
+        lp_join_lanes(t, LP_W);
+        if (lane == 0) s_cta = t;
     }
     if (C > 1) {
         cg::cluster_group cl = cg::this_cluster();
         cl.sync();
         if (rank == 0) {
-            if (tid == 0) {
-                LpStat t = s_cta;
-                for (int c = 1; c < C; ++c) lp_join(t, *cl.map_shared_rank(&s_cta, c));
-                s_stat[0] = t;
+            if (warp == 0) {
+                LpStat t = *cl.map_shared_rank(&s_cta, lane % C);
+                lp_join_lanes(t, C);
+                if (lane == 0) s_stat[0] = t;
             }
             if constexpr (TOP) {
-                // the CTAs' lists one after another; absent keys (0) rank last
+                // ceil(n / C) values of every CTA reach the least of the CTAs' ceil(n / C)-th
+                // ones, n values at least: only what reaches it is ranked
+                const int deep = (a.n_top + C - 1) / C;
+                uint64_t* lists = s_buf;  // done with: every warp has copied its keys
+                if (tid == 0) s_cnt[0] = 0;
                 for (int i = tid; i < C * a.n_top; i += LP_NT) {
-                    const int c = i / a.n_top, j = i - c * a.n_top;
-                    s_all[i] = cl.map_shared_rank(s_best, c)[j];
+                    const int c = i / a.n_top;
+                    lists[i] = cl.map_shared_rank(s_best, c)[i - c * a.n_top];
                 }
+                __syncthreads();
+                uint64_t bound = ~0ull;
+                for (int c = 0; c < C; ++c) {
+                    const uint64_t k = lists[c * a.n_top + deep - 1];
+                    bound = k < bound ? k : bound;
+                }
+                for (int i = tid; i < C * a.n_top; i += LP_NT)
+                    if (lists[i] >= bound && lists[i]) s_all[atomicAdd(&s_cnt[0], 1)] = lists[i];
+                __syncthreads();
+                lp_rank(s_all, s_cnt[0], s_best, a.n_top, tid);
             }
         }
         cl.sync();  // the other CTAs' shared memory stays until it has been read
         if (rank != 0) return;
-        if constexpr (TOP) {
-            if (tid < a.n_top) s_best[tid] = 0;
-            __syncthreads();
-            for (int i = tid; i < C * a.n_top; i += LP_NT) {
-                const uint64_t k = s_all[i];
-                int r = 0;
-                for (int j = 0; j < C * a.n_top; ++j) r += s_all[j] > k;
-                if (k && r < a.n_top) s_best[r] = k;
-            }
-        }
         if (tid == 0) s_cta = s_stat[0];
     }
     __syncthreads();

@@ -15,17 +15,19 @@
 #include "pi_common.cuh"
 #include "pi_internal.h"
 
-#include <cuda_bf16.h>
+#include <cooperative_groups.h>
 
 #include <algorithm>
 #include <exception>
+
+namespace cg = cooperative_groups;
 
 struct pi_proj {
     pi_ctx* ctx = nullptr;
     int qtype = 0;
     int64_t n_in = 0, n_out = 0;
     int64_t groups = 0;  // groups of four 32-element blocks of a row, the last padded with zeros
-    int64_t tiles = 0;   // tiles of 16 rows, an even number, padded with zero rows
+    int64_t tiles = 0;   // tiles of 16 rows, the last padded with zero rows
     uint8_t* w = nullptr;
 };
 
@@ -134,35 +136,63 @@ PI_DEV void ld_adapter8(const void* base, int64_t off, int dtype, float* f) {
 }
 
 // ---------------------------------------------------------------------------
-// k_proj_prep: CTAs 0..T-1 put one token's activations in fragment order (n-tiles of 8
-// tokens; lane 4 (t % 8) + i), the CTAs after them one warp per token and four rank rows
-// of h. Padded blocks of a row are zero; the columns of tokens behind the last one hold
-// whatever the buffer held, and no output reads them (a column of a product depends on
-// that column alone).
-//   Q8_0: xf [block][n-tile][lane]{k 4i.., k 16+4i..}, xs [block][8 n-tiles] scales
-//   Q4_0: xf [block][n-tile][k-step][lane]{hi, hi, lo, lo} (k 8i + 4 step ..), xs [8 n-tiles]
+// Activations in fragment order: [chunk of NT n-tiles of 8 tokens][group of 4 blocks][n-tile],
+// so that a run of groups of one chunk is one contiguous piece. Lane 4 g + i holds token g of
+// the n-tile:
+//   Q8_0: per pair of blocks 512 B, the lane's {k 4i.., k 16+4i..} of either block, then per
+//         pair 64 B of scales, i's {tokens 2i, 2i+1} of either block
+//   Q4_0: per block and k-step (k 8i + 4 step ..) 512 B, the lane's {hi, hi, lo, lo}
+// ---------------------------------------------------------------------------
+template <int QT>
+constexpr int xgroup_bytes() { return QT == PI_QT_Q8_0 ? 2 * 512 + 2 * 64 : 8 * 512; }
+
+// Within a chunk the columns are ordered by adapter, those without one first, so that an
+// n-tile holds few adapters: the column of a token is the number of tokens of its chunk
+// with a smaller (adapter, token). Columns behind the last token keep their places.
+PI_DEV int lora_key(const LoraArgs& L, int64_t t) {
+    const int a = L.ids[t];
+    return a < 0 || a >= L.n ? -1 : a;
+}
+
+// ---------------------------------------------------------------------------
+// k_proj_prep: CTAs 0..T-1 put one token's activations in fragment order; the CTAs after
+// them compute h, four warps per token and four rank rows (each warp a quarter of the
+// row: its loads are then one or two round trips to memory for usual widths). Padded
+// blocks of a row are zero; the columns of tokens behind the last one hold whatever the
+// buffer held, and no output reads them (a column of a product depends on it alone).
+// Q4_0 activations are scaled by a power of two per token, its reciprocal in xs [T].
 // ---------------------------------------------------------------------------
 constexpr int PREP_T = 256;
-constexpr int PREP_R = 4;  // rank rows per warp
-
-PI_DEV float max_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
+constexpr int PREP_R = 4;   // rank rows of a unit
+constexpr int PREP_S = 4;   // warps of a unit
 
 template <int QT>
 __global__ __launch_bounds__(PREP_T) void k_proj_prep(const float* __restrict__ x, int64_t T, int64_t n_in,
-                                                      int64_t groups, int64_t ntt, uint8_t* __restrict__ xf,
+                                                      int64_t groups, int NT, uint8_t* __restrict__ xf,
                                                       float* __restrict__ xs, const LoraArgs L,
                                                       float* __restrict__ h, uint32_t* err) {
     pdl_wait();
     pdl_trigger();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (blockIdx.x < T) {
-        const int64_t t = blockIdx.x, nt = t >> 3;
-        const int g = (int)(t & 7);
+        const int64_t t = blockIdx.x, chunk = t / (8 * NT), c0 = chunk * (8 * NT);
+        int col = (int)(t - c0);
+        if (L.ids) {
+            const int mine = lora_key(L, t), j = col;
+            col = 0;
+            for (int q = 0; q < 8 * NT; q += 32) {
+                bool before = false;
+                if (q + lane < 8 * NT && c0 + q + lane < T) {
+                    const int o = lora_key(L, c0 + q + lane);
+                    before = o < mine || (o == mine && q + lane < j);
+                }
+                col += __popc(__ballot_sync(0xffffffffu, before));
+            }
+        }
+        const int g = col & 7;
         const float* xr = x + t * n_in;
+        uint8_t* xo = xf + (chunk * groups * NT + (col >> 3)) * xgroup_bytes<QT>();
+        const int64_t gstride = (int64_t)NT * xgroup_bytes<QT>();
         if (L.ids && tid == 0) {
             const int a = L.ids[t];
             if (a >= L.n) atomicOr(err, PI_DEVERR_INDEX);
@@ -177,10 +207,11 @@ __global__ __launch_bounds__(PREP_T) void k_proj_prep(const float* __restrict__ 
                 }
                 float sc;
                 const uint32_t q = quad_quant_q8(e, &sc);
-                const int64_t blk = c * 4 + (lane >> 3);
-                const int j = lane & 7;
-                reinterpret_cast<uint32_t*>(xf)[((blk * ntt + nt) * 32 + g * 4 + (j & 3)) * 2 + (j >> 2)] = q;
-                if (j == 0) xs[blk * ntt * 8 + t] = sc;
+                const int b = lane >> 3, j = lane & 7;  // eighth j of the group's block b
+                uint8_t* o = xo + c * gstride;
+                *reinterpret_cast<uint32_t*>(o + (b >> 1) * 512 + (g * 4 + (j & 3)) * 16 + (b & 1) * 8 + (j >> 2) * 4) = q;
+                if (j == 0)
+                    *reinterpret_cast<float*>(o + 1024 + (b >> 1) * 64 + (g >> 1) * 16 + (b & 1) * 8 + (g & 1) * 4) = sc;
             }
         } else {
             __shared__ float s_m[PREP_T / 32];
@@ -200,7 +231,7 @@ __global__ __launch_bounds__(PREP_T) void k_proj_prep(const float* __restrict__ 
             const bool fin = m < INFINITY;
             const float s = fin ? ldexpf(1.0f, ex) : __int_as_float(0x7fffffff);
             if (tid == 0) xs[t] = fin ? ldexpf(1.0f, -ex) : __int_as_float(0x7fffffff);
-            for (int64_t j = tid; j < groups * 16; j += PREP_T) {
+            for (int64_t j = tid; j < groups * 16; j += PREP_T) {  // eight values: lane i = j % 4 of block j / 4
                 float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
                 if (j * 8 < n_in) {
                     const float4 u = *reinterpret_cast<const float4*>(xr + j * 8);
@@ -217,47 +248,55 @@ __global__ __launch_bounds__(PREP_T) void k_proj_prep(const float* __restrict__ 
                     hi[p] = *reinterpret_cast<const uint32_t*>(&a);
                     lo[p] = *reinterpret_cast<const uint32_t*>(&c);
                 }
-                uint4* o = reinterpret_cast<uint4*>(xf) + ((j >> 2) * ntt + nt) * 64 + g * 4 + (j & 3);
-                o[0] = make_uint4(hi[0], hi[1], lo[0], lo[1]);
-                o[32] = make_uint4(hi[2], hi[3], lo[2], lo[3]);
+                uint8_t* o = xo + (j >> 4) * gstride + ((j >> 2) & 3) * 1024 + (g * 4 + (j & 3)) * 16;
+                *reinterpret_cast<uint4*>(o) = make_uint4(hi[0], hi[1], lo[0], lo[1]);
+                *reinterpret_cast<uint4*>(o + 512) = make_uint4(hi[2], hi[3], lo[2], lo[3]);
             }
         }
         return;
     }
     // h[t][r] = scale * (A[a][r] . x[t])
-    const int per = L.R / PREP_R;
-    const int64_t w = (blockIdx.x - T) * (PREP_T / 32) + warp, t = w / per;
-    const int r0 = (int)(w % per) * PREP_R;
-    if (t >= T) return;
-    int rank;
-    const int a = lora_of(L, t, &rank);
-    if (a < 0 || r0 >= rank) return;
-    float acc[PREP_R] = {};
-    const float* xr = x + t * n_in;
-    const int64_t base = ((int64_t)a * L.R + r0) * n_in;
+    __shared__ float s_h[PREP_T / 32][PREP_R];
+    const int per = L.R / PREP_R, part = warp % PREP_S;
+    const int64_t unit = (blockIdx.x - T) * (PREP_T / 32 / PREP_S) + warp / PREP_S, t = unit / per;
+    const int r0 = (int)(unit % per) * PREP_R;
+    int rank = 0, a = -1;
+    if (t < T) a = lora_of(L, t, &rank);
+    const bool live = a >= 0 && r0 < rank;
+    if (live) {
+        float acc[PREP_R] = {};
+        const float* xr = x + t * n_in;
+        const int64_t base = ((int64_t)a * L.R + r0) * n_in;
 #pragma unroll 2
-    for (int64_t k = lane * 8; k < n_in; k += 256) {
-        const float4 u = *reinterpret_cast<const float4*>(xr + k);
-        const float4 v = *reinterpret_cast<const float4*>(xr + k + 4);
+        for (int64_t k = part * 256 + lane * 8; k < n_in; k += 256 * PREP_S) {
+            const float4 u = *reinterpret_cast<const float4*>(xr + k);
+            const float4 v = *reinterpret_cast<const float4*>(xr + k + 4);
+#pragma unroll
+            for (int r = 0; r < PREP_R; ++r) {
+                float f[8];
+                ld_adapter8(L.a, base + r * n_in + k, L.dtype, f);
+                acc[r] = fmaf(f[0], u.x, acc[r]);
+                acc[r] = fmaf(f[1], u.y, acc[r]);
+                acc[r] = fmaf(f[2], u.z, acc[r]);
+                acc[r] = fmaf(f[3], u.w, acc[r]);
+                acc[r] = fmaf(f[4], v.x, acc[r]);
+                acc[r] = fmaf(f[5], v.y, acc[r]);
+                acc[r] = fmaf(f[6], v.z, acc[r]);
+                acc[r] = fmaf(f[7], v.w, acc[r]);
+            }
+        }
 #pragma unroll
         for (int r = 0; r < PREP_R; ++r) {
-            float f[8];
-            ld_adapter8(L.a, base + r * n_in + k, L.dtype, f);
-            acc[r] = fmaf(f[0], u.x, acc[r]);
-            acc[r] = fmaf(f[1], u.y, acc[r]);
-            acc[r] = fmaf(f[2], u.z, acc[r]);
-            acc[r] = fmaf(f[3], u.w, acc[r]);
-            acc[r] = fmaf(f[4], v.x, acc[r]);
-            acc[r] = fmaf(f[5], v.y, acc[r]);
-            acc[r] = fmaf(f[6], v.z, acc[r]);
-            acc[r] = fmaf(f[7], v.w, acc[r]);
+            const float s = warp_sum(acc[r]);
+            if (lane == 0) s_h[warp][r] = s;
         }
     }
-    const float sc = L.scales ? L.scales[a] : 1.0f;
+    __syncthreads();
+    if (live && part == 0 && lane < PREP_R) {
+        float s = 0.0f;
 #pragma unroll
-    for (int r = 0; r < PREP_R; ++r) {
-        const float s = warp_sum(acc[r]);
-        if (lane == 0) h[t * L.R + r0 + r] = s * sc;
+        for (int q = 0; q < PREP_S; ++q) s += s_h[warp + q][lane];
+        h[t * L.R + r0 + lane] = s * (L.scales ? L.scales[a] : 1.0f);
     }
 }
 
@@ -271,35 +310,11 @@ struct ProjArgs {
     const float* h;
     float* y;
     LoraArgs L;
-    int64_t T, n_out, groups, tiles, ntt;
-    int ks;  // warps that share a tile's blocks
+    int64_t T, n_out, groups, tiles;
+    int ks;      // CTAs that share the blocks of their rows
+    int cg;      // groups of a part that are staged together
+    int nchunk;  // such pieces of a part
 };
-
-PI_DEV uint64_t pack2(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-PI_DEV float2 unpack2(uint64_t v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-PI_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-PI_DEV uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-PI_DEV uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 
 // 1.5 * 2^23 as bits: an integer sum below 2^22 added to these bits is the float
 // 1.5 * 2^23 + sum, so accumulating on it replaces the conversion by one subtraction.
@@ -324,197 +339,353 @@ PI_DEV uint32_t nib_pair(uint32_t w, int p) {
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// A lane's words of one group of MT tiles.
-template <int QT, int MT>
+// A lane's words of one group of a tile.
+template <int QT>
 struct GroupRegs {
     static constexpr int NQ = QT == PI_QT_Q8_0 ? 4 : 2;
-    int4 q[MT][NQ];
-    int4 d[MT];
-    PI_DEV void load(const uint8_t* p, int64_t tile_stride, int lane) {
+    int4 q[NQ];
+    int4 d;
+    PI_DEV void load(const uint8_t* p, int lane) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-#pragma unroll
-            for (int i = 0; i < NQ; ++i) q[m][i] = ld_stream(p + m * tile_stride + i * 512 + lane * 16);
-            d[m] = ld_stream(p + m * tile_stride + NQ * 512 + (lane >> 2) * 16);
-        }
+        for (int i = 0; i < NQ; ++i) q[i] = ld_stream(p + i * 512 + lane * 16);
+        d = ld_stream(p + NQ * 512 + (lane >> 2) * 16);
     }
 };
 PI_DEV int word(const int4& v, int i) { return i == 0 ? v.x : (i == 1 ? v.y : (i == 2 ? v.z : v.w)); }
 
-// CTA = 8 warps = 8 / ks sets of MT tiles, each set's blocks split over ks warps; NT n-tiles
-// of 8 tokens (blockIdx.y: which). The weights stream from memory once per 8 NT tokens,
-// the next group's 16-byte loads in flight while the current one is multiplied; the
-// activations' fragments are read through L1, which the weights bypass.
-template <int QT, int MT, int NT>
-__global__ __launch_bounds__(256) void k_proj_gemm(const ProjArgs p) {
-    extern __shared__ __align__(16) float s_red[];  // [warp][MT * NT][4][32] when ks > 1
-    __shared__ int s_id[8 * NT], s_rank[8 * NT];
+PI_DEV void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+PI_DEV uint32_t to_tf32(float v) {
+    uint32_t r;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(v));
+    return r;
+}
+
+PI_DEV void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+constexpr int GEMM_T = 256;
+constexpr int GEMM_W = GEMM_T / 32;
+
+// CTA = 8 warps of 16 rows each; blockIdx.x = the CTA's part of the blocks (the ks CTAs of a
+// cluster share their rows) + ks * the set of 128 rows; blockIdx.y: the chunk of NT n-tiles.
+// The weights stream from memory once per chunk straight into registers, the next group's
+// 16-byte loads in flight while the current one is multiplied; the activations' fragments
+// come through a stage in shared memory that the CTA's warps share, double-buffered where a
+// part does not fit. Splitting over CTAs rather than over a CTA's warps keeps 128 rows to
+// every staged fragment (n_out 12288, T 16, Q4_0: 54 us with the blocks split over the warps).
+//
+// Adapters: for every (adapter, n-tile) that meet, one product of the adapter's rows of B
+// (exact in tf32 for f16 and bf16 weights, two tf32 terms for f32 ones) with h in two tf32
+// terms on the tensor cores; a column takes it only where its token has that adapter, so
+// an adapter's NaN stays with its requests.
+template <int QT, int NT>
+__global__ __launch_bounds__(GEMM_T, 2) void k_proj_gemm(const ProjArgs p) {
+    constexpr int XG = xgroup_bytes<QT>(), GB = group_bytes<QT>(), NC = 8 * NT;
+    extern __shared__ __align__(16) uint8_t s_x[];  // [2][cg][NT] fragment groups, then the sums
+    __shared__ int s_key[NC], s_id[NC], s_rank[NC], s_tok[NC], s_pair[NC], s_npair;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, i4 = lane & 3;
-    const int ks = p.ks, part = warp % ks;
-    const int64_t set = (int64_t)blockIdx.x * (8 / ks) + warp / ks, tile0 = set * MT;
-    const int64_t nt0 = (int64_t)blockIdx.y * NT;
-    const int nnt = (int)min((int64_t)NT, p.ntt - nt0);  // n-tiles of this CTA
-    const int64_t tile_stride = p.groups * group_bytes<QT>();
+    const int ks = p.ks, part = (int)(blockIdx.x % ks);
+    const int64_t tile = (int64_t)(blockIdx.x / ks) * GEMM_W + warp;
+    const int64_t t0 = (int64_t)blockIdx.y * NC;
+    const int ncol = (int)min((int64_t)NC, p.T - t0);
     const int64_t gb = p.groups * part / ks, ge = p.groups * (part + 1) / ks;
-    const bool live = tile0 < p.tiles;
-    const uint8_t* wp = p.w + tile0 * tile_stride + gb * group_bytes<QT>();
-    GroupRegs<QT, MT> cur, nxt;
-    if (live && gb < ge) cur.load(wp, tile_stride, lane);  // constant weights: before the wait
+    const bool live = tile < p.tiles;
+    const uint8_t* wt = p.w + tile * p.groups * GB;
+    GroupRegs<QT> ra, rb;
+    if (live && gb < ge) ra.load(wt + gb * GB, lane);  // constant weights: before the wait
     pdl_wait();
     pdl_trigger();
-    for (int j = tid; j < 8 * NT; j += 256) {
-        const int64_t t = nt0 * 8 + j;
-        int rank = 0;
-        s_id[j] = (p.L.ids && t < p.T) ? lora_of(p.L, t, &rank) : -1;
-        s_rank[j] = rank;
-    }
-    uint64_t acc[MT][NT][2];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) acc[m][n][0] = acc[m][n][1] = 0;
-    if (live) {
-        for (int64_t gr = gb; gr < ge; ++gr) {
-            wp += group_bytes<QT>();
-            if (gr + 1 < ge) nxt.load(wp, tile_stride, lane);
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                uint64_t dg[MT][2];  // {d, d} of rows g and g + 8
-#pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    const int w = word(cur.d[m], b);
-                    const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&w));
-                    dg[m][0] = pack2(d.x, d.x);
-                    dg[m][1] = pack2(d.y, d.y);
-                }
-                const int64_t blk = gr * 4 + b;
-                if constexpr (QT == PI_QT_Q8_0) {
-                    const uint2* xb = reinterpret_cast<const uint2*>(p.xf) + (blk * p.ntt + nt0) * 32 + lane;
-                    const uint64_t* db = reinterpret_cast<const uint64_t*>(p.xs + (blk * p.ntt + nt0) * 8 + 2 * i4);
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        if (n >= nnt) break;
-                        const uint2 xv = xb[n * 32];
-                        const uint64_t dx = db[n * 4];
-#pragma unroll
-                        for (int m = 0; m < MT; ++m) {
-                            int c[4];
-                            mma_s8(c, *reinterpret_cast<const uint4*>(&cur.q[m][b]), xv);
-                            const uint64_t bias = pack2(-FLOAT_BIAS, -FLOAT_BIAS);
-                            const uint64_t f0 = add2(pack2(__int_as_float(c[0]), __int_as_float(c[1])), bias);
-                            const uint64_t f1 = add2(pack2(__int_as_float(c[2]), __int_as_float(c[3])), bias);
-                            acc[m][n][0] = fma2(f0, mul2(dg[m][0], dx), acc[m][n][0]);
-                            acc[m][n][1] = fma2(f1, mul2(dg[m][1], dx), acc[m][n][1]);
-                        }
-                    }
-                } else {
-                    uint32_t a[MT][2][4];
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) {
-                        const uint32_t w0 = word(cur.q[m][b >> 1], 2 * (b & 1));
-                        const uint32_t w1 = word(cur.q[m][b >> 1], 2 * (b & 1) + 1);
-#pragma unroll
-                        for (int s = 0; s < 2; ++s) {
-                            a[m][s][0] = nib_pair(w0, 2 * s);
-                            a[m][s][1] = nib_pair(w1, 2 * s);
-                            a[m][s][2] = nib_pair(w0, 2 * s + 1);
-                            a[m][s][3] = nib_pair(w1, 2 * s + 1);
-                        }
-                    }
-                    const uint4* xb = reinterpret_cast<const uint4*>(p.xf) + (blk * p.ntt + nt0) * 64 + lane;
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        if (n >= nnt) break;
-                        const uint4 x0 = xb[n * 64], x1 = xb[n * 64 + 32];
-#pragma unroll
-                        for (int m = 0; m < MT; ++m) {
-                            float c[4] = {0.f, 0.f, 0.f, 0.f};
-                            mma_f16(c, a[m][0], x0.z, x0.w);
-                            mma_f16(c, a[m][1], x1.z, x1.w);
-                            mma_f16(c, a[m][0], x0.x, x0.y);
-                            mma_f16(c, a[m][1], x1.x, x1.y);
-                            acc[m][n][0] = fma2(dg[m][0], pack2(c[0], c[1]), acc[m][n][0]);
-                            acc[m][n][1] = fma2(dg[m][1], pack2(c[2], c[3]), acc[m][n][1]);
-                        }
-                    }
-                }
+
+    const uint8_t* xsrc = p.xf + (int64_t)blockIdx.y * p.groups * (NT * XG);
+    const uint32_t s_base = (uint32_t)__cvta_generic_to_shared(s_x);
+    const int stage_bytes = p.cg * (NT * XG);
+    auto stage = [&](int c) {
+        const int64_t b = gb + (int64_t)c * p.cg, e = min(ge, b + p.cg);
+        const int n16 = (int)(max((int64_t)0, e - b) * (NT * XG / 16));
+        const uint32_t dst = s_base + (c & 1) * stage_bytes;
+        const uint8_t* src = xsrc + b * (NT * XG);
+        for (int i = tid; i < n16; i += GEMM_T) cp_async16(dst + i * 16, src + i * 16);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    stage(0);
+    if (p.L.ids) {
+        for (int j = tid; j < ncol; j += GEMM_T) s_key[j] = lora_key(p.L, t0 + j);
+        __syncthreads();
+        for (int j = tid; j < NC; j += GEMM_T) {
+            int col = j, a = -1, rank = 0;
+            if (j < ncol) {
+                a = s_key[j];
+                col = 0;
+                for (int q = 0; q < ncol; ++q) col += s_key[q] < a || (s_key[q] == a && q < j);
+                if (a >= 0) lora_of(p.L, t0 + j, &rank);
             }
-            cur = nxt;
+            s_id[col] = a;
+            s_rank[col] = rank;
+            s_tok[col] = j;
         }
-    }
-    if (ks > 1) {
-        float* mine = s_red + (size_t)warp * (MT * NT * 128) + lane;
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                if (n >= nnt) break;
-                const float2 u = unpack2(acc[m][n][0]), v = unpack2(acc[m][n][1]);
-                float* o = mine + (m * NT + n) * 128;
-                o[0] = u.x;
-                o[32] = u.y;
-                o[64] = v.x;
-                o[96] = v.y;
+        __syncthreads();
+        if (warp == 0) {  // the (adapter, n-tile) pairs, each by its first column
+            int n = 0;
+            for (int q = 0; q < NC; q += 32) {
+                const int j = q + lane;
+                const bool start = j < NC && s_id[j] >= 0 && s_rank[j] > 0 && (j >> 3) % ks == part &&
+                                   ((j & 7) == 0 || s_id[j - 1] != s_id[j]);
+                const uint32_t b = __ballot_sync(0xffffffffu, start);
+                if (start) s_pair[n + __popc(b & ((1u << lane) - 1u))] = j;
+                n += __popc(b);
             }
+            if (lane == 0) s_npair = n;
+        }
+    } else {
+        for (int j = tid; j < NC; j += GEMM_T) s_tok[j] = j;
+        if (tid == 0) s_npair = 0;
     }
-    __syncthreads();
-    if (!live) return;
+
+    uint64_t sum[NT][2];  // pairs of neighbouring columns, rows g and g + 8
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int n = 0; n < NT; ++n) sum[n][0] = sum[n][1] = 0;
+    auto multiply = [&](const GroupRegs<QT>& w, const uint8_t* xg) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            if (n >= nnt) break;
-            if (ks > 1 && n % ks != part) continue;
-            float c[2][2];  // [row g / g + 8][token 2 i4, 2 i4 + 1]
-            if (ks > 1) {
-                const float* from = s_red + (size_t)(warp - part) * (MT * NT * 128) + (m * NT + n) * 128 + lane;
+        for (int hb = 0; hb < 2; ++hb) {  // two blocks at a time
+            uint64_t dg[2][2];            // [block]{d, d} of rows g and g + 8
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float s = 0.0f;
-                    for (int q = 0; q < ks; ++q) s += from[(size_t)q * (MT * NT * 128) + j * 32];
-                    c[j >> 1][j & 1] = s;
+            for (int b = 0; b < 2; ++b) {
+                const int v = word(w.d, 2 * hb + b);
+                const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&v));
+                dg[b][0] = pack2(d.x, d.x);
+                dg[b][1] = pack2(d.y, d.y);
+            }
+            if constexpr (QT == PI_QT_Q8_0) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const uint4 xv = *reinterpret_cast<const uint4*>(xg + n * XG + hb * 512 + lane * 16);
+                    const ulonglong2 dx = *reinterpret_cast<const ulonglong2*>(xg + n * XG + 1024 + hb * 64 + i4 * 16);
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        int s[4];
+                        mma_s8(s, *reinterpret_cast<const uint4*>(&w.q[2 * hb + b]),
+                               b ? make_uint2(xv.z, xv.w) : make_uint2(xv.x, xv.y));
+                        const uint64_t bias = pack2(-FLOAT_BIAS, -FLOAT_BIAS), d2 = b ? dx.y : dx.x;
+                        const uint64_t f0 = add2(pack2(__int_as_float(s[0]), __int_as_float(s[1])), bias);
+                        const uint64_t f1 = add2(pack2(__int_as_float(s[2]), __int_as_float(s[3])), bias);
+                        sum[n][0] = fma2(f0, mul2(dg[b][0], d2), sum[n][0]);
+                        sum[n][1] = fma2(f1, mul2(dg[b][1], d2), sum[n][1]);
+                    }
                 }
             } else {
-                const float2 u = unpack2(acc[m][n][0]), v = unpack2(acc[m][n][1]);
-                c[0][0] = u.x;
-                c[0][1] = u.y;
-                c[1][0] = v.x;
-                c[1][1] = v.y;
-            }
-            const int64_t row = (tile0 + m) * 16 + g;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int j = n * 8 + 2 * i4 + e;
-                const int64_t t = nt0 * 8 + j;
-                if (t >= p.T) continue;
-                if (QT == PI_QT_Q4_0) {
-                    const float s = p.xs[t];
-                    c[0][e] *= s;
-                    c[1][e] *= s;
-                }
-                const int a = s_id[j], rank = s_rank[j];
-                if (a >= 0) {
-                    const float* h = p.h + t * p.L.R;
-                    for (int r = 0; r < rank; r += 8) {
-                        float hv[8];
+                for (int b = 0; b < 2; ++b) {
+                    uint32_t a[2][4];
+                    const uint32_t w0 = word(w.q[hb], 2 * b), w1 = word(w.q[hb], 2 * b + 1);
 #pragma unroll
-                        for (int q = 0; q < 8; ++q) hv[q] = r + q < rank ? h[r + q] : 0.0f;
+                    for (int s = 0; s < 2; ++s) {
+                        a[s][0] = nib_pair(w0, 2 * s);
+                        a[s][1] = nib_pair(w1, 2 * s);
+                        a[s][2] = nib_pair(w0, 2 * s + 1);
+                        a[s][3] = nib_pair(w1, 2 * s + 1);
+                    }
 #pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            if (row + 8 * k >= p.n_out) continue;
-                            float f[8];
-                            ld_adapter8(p.L.b, ((int64_t)a * p.n_out + row + 8 * k) * p.L.R + r, p.L.dtype, f);
-#pragma unroll
-                            for (int q = 0; q < 8; ++q)
-                                if (r + q < rank) c[k][e] = fmaf(f[q], hv[q], c[k][e]);
-                        }
+                    for (int n = 0; n < NT; ++n) {
+                        const uint8_t* xb = xg + n * XG + (2 * hb + b) * 1024 + lane * 16;
+                        const uint4 x0 = *reinterpret_cast<const uint4*>(xb);
+                        const uint4 x1 = *reinterpret_cast<const uint4*>(xb + 512);
+                        float s[4] = {0.f, 0.f, 0.f, 0.f};
+                        mma_f16(s, a[0], x0.z, x0.w);
+                        mma_f16(s, a[1], x1.z, x1.w);
+                        mma_f16(s, a[0], x0.x, x0.y);
+                        mma_f16(s, a[1], x1.x, x1.y);
+                        sum[n][0] = fma2(dg[b][0], pack2(s[0], s[1]), sum[n][0]);
+                        sum[n][1] = fma2(dg[b][1], pack2(s[2], s[3]), sum[n][1]);
                     }
                 }
-#pragma unroll
-                for (int k = 0; k < 2; ++k)
-                    if (row + 8 * k < p.n_out) p.y[t * p.n_out + row + 8 * k] = c[k][e];
             }
         }
+    };
+    for (int c = 0; c < p.nchunk; ++c) {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();  // piece c has landed; nobody reads the other buffer any more
+        if (c + 1 < p.nchunk) stage(c + 1);
+        if (!live) continue;
+        const uint8_t* xg = s_x + (c & 1) * stage_bytes;
+        const int64_t g0 = gb + (int64_t)c * p.cg, g1 = min(ge, g0 + p.cg);
+        // two register sets in turn; a piece that is not the last has an even number of groups
+#pragma unroll 1
+        for (int64_t gr = g0; gr < g1; gr += 2, xg += 2 * NT * XG) {
+            if (gr + 1 < ge) rb.load(wt + (gr + 1) * GB, lane);
+            multiply(ra, xg);
+            if (gr + 1 >= g1) break;
+            if (gr + 2 < ge) ra.load(wt + (gr + 2) * GB, lane);
+            multiply(rb, xg + NT * XG);
+        }
+    }
+    float acc[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const float2 u = unpack2(sum[n][0]), v = unpack2(sum[n][1]);
+        acc[n][0] = u.x;
+        acc[n][1] = u.y;
+        acc[n][2] = v.x;
+        acc[n][3] = v.y;
+    }
+    if (ks > 1) {  // n-tile n belongs to CTA n % ks of the cluster from here on
+        cg::cluster_group cl = cg::this_cluster();
+        float* sums = reinterpret_cast<float*>(s_x);
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+            *reinterpret_cast<float4*>(sums + ((warp * NT + n) * 32 + lane) * 4) =
+                make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
+        cl.sync();
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            if (n % ks != part) continue;
+            float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int q = 0; q < ks; ++q) {
+                const float4 v =
+                    *reinterpret_cast<const float4*>(cl.map_shared_rank(sums, q) + ((warp * NT + n) * 32 + lane) * 4);
+                t.x += v.x;
+                t.y += v.y;
+                t.z += v.z;
+                t.w += v.w;
+            }
+            acc[n][0] = t.x;
+            acc[n][1] = t.y;
+            acc[n][2] = t.z;
+            acc[n][3] = t.w;
+        }
+        cl.sync();  // the other CTAs' shared memory stays until it has been read
+    }
+    if (!live) return;
+    if (QT == PI_QT_Q4_0) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int u = n * 8 + 2 * i4;
+            const float su = u < ncol ? p.xs[t0 + s_tok[u]] : 0.0f, sv = u + 1 < ncol ? p.xs[t0 + s_tok[u + 1]] : 0.0f;
+            acc[n][0] *= su;
+            acc[n][1] *= sv;
+            acc[n][2] *= su;
+            acc[n][3] *= sv;
+        }
+    }
+    const int npair = s_npair;
+    if (npair) {
+        struct Item {
+            uint4 b[2];  // four rank entries of rows g and g + 8 as they are stored
+            float4 h;
+        } cur, nxt;
+        auto fetch = [&](Item& it, int i, int r0) {
+            const int j = s_pair[i], a = s_id[j], r = r0 + 4 * i4;
+            const bool in = r < s_rank[j];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int64_t row = tile * 16 + g + 8 * k, off = ((int64_t)a * p.n_out + row) * p.L.R + r;
+                it.b[k] = make_uint4(0, 0, 0, 0);
+                if (in && row < p.n_out) {
+                    if (p.L.dtype == PI_QT_F32) {
+                        it.b[k] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(p.L.b) + off));
+                    } else {
+                        const uint2 v = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p.L.b) + off));
+                        it.b[k].x = v.x;
+                        it.b[k].y = v.y;
+                    }
+                }
+            }
+            const int col = (j & ~7) + g;
+            it.h = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (in && s_id[col] == a) it.h = *reinterpret_cast<const float4*>(p.h + (t0 + s_tok[col]) * p.L.R + r);
+        };
+        float c[4] = {0.f, 0.f, 0.f, 0.f};
+        int i = 0, r0 = 0;
+        fetch(cur, 0, 0);
+        while (i < npair) {
+            const int j = s_pair[i], rank = s_rank[j], a = s_id[j];
+            const bool last = r0 + 16 >= rank;
+            const int ni = last ? i + 1 : i, nr = last ? 0 : r0 + 16;
+            if (ni < npair) fetch(nxt, ni, nr);
+            const int left = rank - r0 - 4 * i4;  // rank entries of this lane's four that count
+            float bv[2][4];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const uint4 v = cur.b[k];
+                if (p.L.dtype == PI_QT_F32) {
+                    bv[k][0] = __uint_as_float(v.x);
+                    bv[k][1] = __uint_as_float(v.y);
+                    bv[k][2] = __uint_as_float(v.z);
+                    bv[k][3] = __uint_as_float(v.w);
+                } else if (p.L.dtype == PI_QT_F16) {
+                    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&v.x));
+                    const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
+                    bv[k][0] = x.x;
+                    bv[k][1] = x.y;
+                    bv[k][2] = y.x;
+                    bv[k][3] = y.y;
+                } else {
+                    bv[k][0] = __uint_as_float(v.x << 16);
+                    bv[k][1] = __uint_as_float(v.x & 0xffff0000u);
+                    bv[k][2] = __uint_as_float(v.y << 16);
+                    bv[k][3] = __uint_as_float(v.y & 0xffff0000u);
+                }
+            }
+            const float hv[4] = {cur.h.x, cur.h.y, cur.h.z, cur.h.w};
+            uint32_t big[2][4], small[2][4], hb[4], hs[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float h = q < left ? hv[q] : 0.0f;
+                hb[q] = to_tf32(h);
+                hs[q] = to_tf32(h - __uint_as_float(hb[q]));
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const float f = q < left ? bv[k][q] : 0.0f;
+                    big[q >> 1][k + 2 * (q & 1)] = to_tf32(f);
+                    small[q >> 1][k + 2 * (q & 1)] = to_tf32(f - __uint_as_float(to_tf32(f)));
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                if (p.L.dtype == PI_QT_F32) mma_tf32(c, small[s], hb[2 * s], hb[2 * s + 1]);
+                mma_tf32(c, big[s], hs[2 * s], hs[2 * s + 1]);
+                mma_tf32(c, big[s], hb[2 * s], hb[2 * s + 1]);
+            }
+            if (last) {
+                const int n0 = j >> 3;
+                const bool u0 = s_id[n0 * 8 + 2 * i4] == a, u1 = s_id[n0 * 8 + 2 * i4 + 1] == a;
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    if (n == n0) {
+                        if (u0) {
+                            acc[n][0] += c[0];
+                            acc[n][2] += c[2];
+                        }
+                        if (u1) {
+                            acc[n][1] += c[1];
+                            acc[n][3] += c[3];
+                        }
+                    }
+                c[0] = c[1] = c[2] = c[3] = 0.0f;
+            }
+            cur = nxt;
+            i = ni;
+            r0 = nr;
+        }
+    }
+    const int64_t row = tile * 16 + g;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        if (ks > 1 && n % ks != part) continue;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int col = n * 8 + 2 * i4 + e;
+            if (col >= ncol) continue;
+            float* y = p.y + (t0 + s_tok[col]) * p.n_out + row;
+            if (row < p.n_out) y[0] = acc[n][e];
+            if (row + 8 < p.n_out) y[8] = acc[n][2 + e];
+        }
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -527,12 +698,18 @@ struct ProjBufs {
     float *xs, *h;
     size_t bytes;
 };
+// n-tiles of 8 tokens are worked on in chunks of up to 8, as even as they come
+int proj_chunk(int64_t T) {
+    const int64_t ntt = (T + 7) / 8, chunks = (ntt + 7) / 8;
+    return (int)((ntt + chunks - 1) / chunks);
+}
 ProjBufs proj_carve(const pi_proj* P, int64_t T, int64_t R, char* base) {
     PiBump b{base};
     ProjBufs o;
-    const int64_t ntt = (T + 7) / 8, blocks = P->groups * 4;
-    o.xf = b.take<uint8_t>((size_t)(blocks * ntt) * (P->qtype == PI_QT_Q8_0 ? 256 : 1024));
-    o.xs = b.take<float>((size_t)(ntt * 8) * (P->qtype == PI_QT_Q8_0 ? blocks : 1));
+    const int64_t NT = proj_chunk(T), chunks = ((T + 7) / 8 + NT - 1) / NT;
+    const int64_t xg = P->qtype == PI_QT_Q8_0 ? xgroup_bytes<PI_QT_Q8_0>() : xgroup_bytes<PI_QT_Q4_0>();
+    o.xf = b.take<uint8_t>((size_t)(chunks * P->groups * NT * xg));
+    o.xs = b.take<float>((size_t)(P->qtype == PI_QT_Q4_0 ? T : 0));
     o.h = b.take<float>((size_t)(T * R));
     o.bytes = b.off + 256;
     return o;
@@ -582,7 +759,7 @@ int proj_create(pi_ctx* ctx, const void* raw, uint64_t raw_len, int32_t qtype, i
     P->n_in = n_in;
     P->n_out = n_out;
     P->groups = (n_in / 32 + 3) / 4;
-    P->tiles = ((n_out + 15) / 16 + 1) & ~(int64_t)1;
+    P->tiles = (n_out + 15) / 16;
     const int64_t gbytes = qtype == PI_QT_Q8_0 ? group_bytes<PI_QT_Q8_0>() : group_bytes<PI_QT_Q4_0>();
     if (P->tiles * P->groups > INT32_MAX) {
         delete P;
@@ -602,33 +779,60 @@ int proj_create(pi_ctx* ctx, const void* raw, uint64_t raw_len, int32_t qtype, i
     return PI_OK;
 }
 
-template <int QT, int MT, int NT>
-void launch_gemm(const ProjArgs& a, cudaStream_t st) {
-    const size_t smem = a.ks > 1 ? sizeof(float) * 8 * MT * NT * 128 : 0;
-    pi_smem_attr((const void*)k_proj_gemm<QT, MT, NT>, smem);
-    const int64_t per = (int64_t)MT * (8 / a.ks);
-    pi_pdl_launch(k_proj_gemm<QT, MT, NT>,
-                  dim3((unsigned)((a.tiles + per - 1) / per), (unsigned)((a.ntt + NT - 1) / NT)), dim3(256), smem, st, a);
+template <int QT, int NT>
+cudaError_t launch_gemm(ProjArgs a, int64_t sms, cudaStream_t st) {
+    constexpr int XG = NT * xgroup_bytes<QT>();
+    const int64_t sets = (a.tiles + GEMM_W - 1) / GEMM_W, chunks = ((a.T + 8 * NT - 1) / (8 * NT));
+    // Parts of the blocks: the time is about the rounds of CTAs, two to an SM, times the groups
+    // of a part plus what a CTA costs beside them (start, stage and join, about six groups)
+    a.ks = 1;
+    int64_t best = INT64_MAX;
+    for (int ks = 1; ks <= 8 && ks <= a.groups; ++ks) {
+        const int64_t rounds = (sets * chunks * ks + 2 * sms - 1) / (2 * sms);
+        const int64_t cost = rounds * ((a.groups + ks - 1) / ks + 6);
+        if (cost < best) {
+            best = cost;
+            a.ks = ks;
+        }
+    }
+    // A part is staged whole where two CTAs of an SM have room for it, in pieces of an even
+    // number of groups otherwise
+    const int64_t budget = 100 * 1024, part = (a.groups + a.ks - 1) / a.ks;
+    a.cg = (int)part;
+    if (part * XG > budget) a.cg = (int)std::max<int64_t>(2, budget / 2 / XG / 2 * 2);
+    a.nchunk = (int)((part + a.cg - 1) / a.cg);
+    const size_t sums = a.ks > 1 ? (size_t)GEMM_W * NT * 512 : 0;
+    const size_t smem = std::max<size_t>((size_t)std::min(a.nchunk, 2) * a.cg * XG, sums);
+    auto kern = k_proj_gemm<QT, NT>;
+    pi_smem_attr((const void*)kern, smem);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(sets * a.ks), (unsigned)chunks);
+    cfg.blockDim = dim3(GEMM_T);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = (unsigned)a.ks;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = a.ks > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kern, a);
 }
 
 template <int QT>
-void dispatch_gemm(ProjArgs a, int64_t sms, cudaStream_t st) {
-    // Two tiles per warp halve the activation reads from L1, which bound batches of more
-    // than 16 tokens, where enough tiles are left to fill the SMs with 8 warps each
-    if (a.ntt > 2 && a.tiles / 2 >= 8 * sms) {
-        a.ks = 1;
-        if (a.ntt <= 4) launch_gemm<QT, 2, 4>(a, st);
-        else launch_gemm<QT, 2, 8>(a, st);
-        return;
+cudaError_t dispatch_gemm(const ProjArgs& a, int NT, int64_t sms, cudaStream_t st) {
+    switch (NT) {
+        case 1: return launch_gemm<QT, 1>(a, sms, st);
+        case 2: return launch_gemm<QT, 2>(a, sms, st);
+        case 3: return launch_gemm<QT, 3>(a, sms, st);
+        case 4: return launch_gemm<QT, 4>(a, sms, st);
+        case 5: return launch_gemm<QT, 5>(a, sms, st);
+        case 6: return launch_gemm<QT, 6>(a, sms, st);
+        case 7: return launch_gemm<QT, 7>(a, sms, st);
+        default: return launch_gemm<QT, 8>(a, sms, st);
     }
-    // Few rows: a tile's blocks are split over up to eight warps, until 16 warps per SM
-    // have work
-    a.ks = 1;
-    while (a.ks < 8 && a.tiles * a.ks < 16 * sms && a.groups >= 2 * a.ks) a.ks *= 2;
-    if (a.ntt <= 1) launch_gemm<QT, 1, 1>(a, st);
-    else if (a.ntt <= 2) launch_gemm<QT, 1, 2>(a, st);
-    else if (a.ntt <= 4) launch_gemm<QT, 1, 4>(a, st);
-    else launch_gemm<QT, 1, 8>(a, st);
 }
 
 int check_bank(pi_ctx* ctx, const pi_lora_bank* bank, const int32_t* ids) {
@@ -663,23 +867,23 @@ int proj_forward(pi_ctx* ctx, const pi_proj* P, const float* x, int64_t T, const
     LoraArgs L = {};
     if (bank) L = LoraArgs{bank->a, bank->b, bank->ranks, bank->scales, ids, bank->dtype, bank->n_adapters, (int)R};
     const bool q8 = P->qtype == PI_QT_Q8_0;
-    const int64_t ntt = (T + 7) / 8;
+    const int NT = proj_chunk(T);
     {
         PiProfScope ps(ctx, st, "k_proj_prep");
-        const int64_t warps = T * (R / PREP_R), grid = T + (warps + PREP_T / 32 - 1) / (PREP_T / 32);
+        const int64_t units = T * (R / PREP_R), per = PREP_T / 32 / PREP_S, grid = T + (units + per - 1) / per;
         if (q8)
             pi_pdl_launch(k_proj_prep<PI_QT_Q8_0>, dim3((unsigned)grid), dim3(PREP_T), 0, st, x, T, P->n_in, P->groups,
-                          ntt, B.xf, B.xs, L, B.h, ctx->dev_err);
+                          NT, B.xf, B.xs, L, B.h, ctx->dev_err);
         else
             pi_pdl_launch(k_proj_prep<PI_QT_Q4_0>, dim3((unsigned)grid), dim3(PREP_T), 0, st, x, T, P->n_in, P->groups,
-                          ntt, B.xf, B.xs, L, B.h, ctx->dev_err);
+                          NT, B.xf, B.xs, L, B.h, ctx->dev_err);
     }
     {
         PiProfScope ps(ctx, st, "k_proj_gemm");
-        const ProjArgs a{P->w, B.xf, B.xs, B.h, y, L, T, P->n_out, P->groups, P->tiles, ntt, 1};
+        const ProjArgs a{P->w, B.xf, B.xs, B.h, y, L, T, P->n_out, P->groups, P->tiles, 1, 1, 1};
         const int64_t sms = ctx->sm_count > 0 ? ctx->sm_count : 148;
-        if (q8) dispatch_gemm<PI_QT_Q8_0>(a, sms, st);
-        else dispatch_gemm<PI_QT_Q4_0>(a, sms, st);
+        const cudaError_t e = q8 ? dispatch_gemm<PI_QT_Q8_0>(a, NT, sms, st) : dispatch_gemm<PI_QT_Q4_0>(a, NT, sms, st);
+        if (e != cudaSuccess) return pi_cuda_check(ctx, e, "projection");
     }
     return pi_cuda_check(ctx, cudaGetLastError(), "projection") ? PI_ERR_CUDA : PI_OK;
 }
