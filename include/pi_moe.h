@@ -200,6 +200,18 @@ int pi_moe_forward(pi_ctx* ctx, pi_moe_layer* layer, const float* x, int64_t T, 
 int pi_moe_forward_routed(pi_ctx* ctx, pi_moe_layer* layer, const float* x, int64_t T, float* out, int32_t flags,
                           int32_t* idx, float* gates, int32_t* counts, int32_t* offsets, int32_t* perm, void* stream);
 
+/* pi_moe_forward for a few tokens in two kernels (model/mod.rs:1239-1633): a decode batch
+ * of T <= 16 tokens through a Q4_0 layer that holds all its experts. Routing is that of
+ * pi_moe_route bit for bit; outputs equal pi_moe_forward's to f32 rounding (block sums in
+ * another order). flags: PI_FWD_RMSNORM | PI_FWD_RESIDUAL. x and out 16-byte aligned; out
+ * may be x. workspace: pi_moe_fused_workspace(layer, T) bytes, 256-byte aligned, that
+ * nothing else uses until the call's work is done (two captured graphs need one each);
+ * NULL: the stream's scratch arena (pi_ctx_reserve before a capture). The second kernel
+ * is a cooperative launch of one CTA per SM, so such calls on several streams take turns. */
+uint64_t pi_moe_fused_workspace(const pi_moe_layer* layer, int64_t T);
+int pi_moe_forward_fused(pi_ctx* ctx, const pi_moe_layer* layer, const float* x, int64_t T, float* out, int32_t flags,
+                         void* workspace, uint64_t workspace_bytes, void* stream);
+
 /* ---- Expert parallelism (config 5: experts sharded over the GPUs of a box) ----
  * No reference counterpart: the reference runs the whole layer in one process
  * (model/mod.rs:1245-1571). These calls split pi_moe_forward into the stages

@@ -26,7 +26,7 @@ struct pi_proj {
     pi_ctx* ctx = nullptr;
     int qtype = 0;
     int64_t n_in = 0, n_out = 0;
-    int64_t groups = 0;  // groups of four 32-element blocks of a row, the last padded with zeros
+    int64_t units = 0;   // pairs of 32-element blocks of a row, the last padded with zeros
     int64_t tiles = 0;   // tiles of 16 rows, the last padded with zero rows
     uint8_t* w = nullptr;
 };
@@ -34,32 +34,32 @@ struct pi_proj {
 namespace {
 
 // ---------------------------------------------------------------------------
-// Weights in fragment order: [tile of 16 rows][group of 4 blocks], a group being one
-// contiguous run that the 32 lanes read with 16-byte loads. Lane 4 g + i holds rows g and
-// g + 8 of the tile:
-//   Q8_0: 4 x 512 B, per block the lane's {row g: k 4i.., row g+8: k 4i.., row g: k 16+4i..,
+// Weights in fragment order: [tile of 16 rows][unit of 2 blocks], a unit being one contiguous
+// run that the 32 lanes read with 16-byte loads. Lane 4 g + i holds rows g and g + 8 of the
+// tile:
+//   Q8_0: 2 x 512 B, per block the lane's {row g: k 4i.., row g+8: k 4i.., row g: k 16+4i..,
 //         row g+8: k 16+4i..} (the A registers of m16n8k32)
-//   Q4_0: 2 x 512 B, per two blocks the lane's {row g, row g+8} words of k 8i..8i+7, the
-//         nibble of k = 8i + 2p (+1) at bits 4p (16 + 4p): one mask then gives a pair of
-//         neighbours in the two halves of a register
-//   then 128 B of scales: [g][block]{d of row g, d of row g+8} in f16
+//   Q4_0: 512 B, per block the lane's {row g, row g+8} words of k 8i..8i+7, the nibble of
+//         k = 8i + 2p (+1) at bits 4p (16 + 4p): one mask then gives a pair of neighbours
+//         in the two halves of a register
+//   then 64 B of scales: [g][block]{d of row g, d of row g+8} in f16
 // ---------------------------------------------------------------------------
 template <int QT>
-constexpr int group_bytes() { return (QT == PI_QT_Q8_0 ? 2048 : 1024) + 128; }
+constexpr int unit_bytes() { return (QT == PI_QT_Q8_0 ? 1024 : 512) + 64; }
 
 PI_DEV uint32_t ld_u16x2(const uint8_t* p) {  // GGUF blocks are 2-byte aligned
     const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
     return q[0] | ((uint32_t)q[1] << 16);
 }
 
-// One thread per (tile, group, block, lane); raw holds rows [row0, row0 + rows).
+// One thread per (tile, unit, block, lane); raw holds n_rows rows.
 template <int QT>
-__global__ __launch_bounds__(128) void k_proj_pack(const uint8_t* __restrict__ raw, int64_t nb, int64_t n_rows,
-                                                   int64_t groups, uint8_t* __restrict__ dst) {
-    const int b4 = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, i = lane & 3;
-    const int64_t tile = blockIdx.x / groups, grp = blockIdx.x % groups, b = grp * 4 + b4;
+__global__ __launch_bounds__(64) void k_proj_pack(const uint8_t* __restrict__ raw, int64_t nb, int64_t n_rows,
+                                                  int64_t units, uint8_t* __restrict__ dst) {
+    const int b2 = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, i = lane & 3;
+    const int64_t tile = blockIdx.x / units, unit = blockIdx.x % units, b = unit * 2 + b2;
     constexpr int BB = QT == PI_QT_Q8_0 ? 34 : 18;
-    uint8_t* out = dst + (int64_t)blockIdx.x * group_bytes<QT>();
+    uint8_t* out = dst + (int64_t)blockIdx.x * unit_bytes<QT>();
     uint32_t w[2][2] = {{0, 0}, {0, 0}};  // [row g / g + 8][word]
     uint16_t d[2] = {0, 0};
 #pragma unroll
@@ -82,13 +82,12 @@ __global__ __launch_bounds__(128) void k_proj_pack(const uint8_t* __restrict__ r
         }
     }
     if (QT == PI_QT_Q8_0) {
-        *reinterpret_cast<uint4*>(out + b4 * 512 + lane * 16) = make_uint4(w[0][0], w[1][0], w[0][1], w[1][1]);
+        *reinterpret_cast<uint4*>(out + b2 * 512 + lane * 16) = make_uint4(w[0][0], w[1][0], w[0][1], w[1][1]);
     } else {
-        *reinterpret_cast<uint2*>(out + (b4 >> 1) * 512 + lane * 16 + (b4 & 1) * 8) = make_uint2(w[0][0], w[1][0]);
+        *reinterpret_cast<uint2*>(out + lane * 16 + b2 * 8) = make_uint2(w[0][0], w[1][0]);
     }
     if (i == 0)
-        *reinterpret_cast<uint32_t*>(out + group_bytes<QT>() - 128 + g * 16 + b4 * 4) =
-            d[0] | ((uint32_t)d[1] << 16);
+        *reinterpret_cast<uint32_t*>(out + unit_bytes<QT>() - 64 + g * 8 + b2 * 4) = d[0] | ((uint32_t)d[1] << 16);
 }
 
 // ---------------------------------------------------------------------------
@@ -136,15 +135,21 @@ PI_DEV void ld_adapter8(const void* base, int64_t off, int dtype, float* f) {
 }
 
 // ---------------------------------------------------------------------------
-// Activations in fragment order: [chunk of NT n-tiles of 8 tokens][group of 4 blocks][n-tile],
-// so that a run of groups of one chunk is one contiguous piece. Lane 4 g + i holds token g of
+// Activations in fragment order: [chunk of NT n-tiles of 8 tokens][unit of 2 blocks][n-tile],
+// so that a run of units of one chunk is one contiguous piece. Lane 4 g + i holds token g of
 // the n-tile:
-//   Q8_0: per pair of blocks 512 B, the lane's {k 4i.., k 16+4i..} of either block, then per
-//         pair 64 B of scales, i's {tokens 2i, 2i+1} of either block
+//   Q8_0: 512 B, the lane's {k 4i.., k 16+4i..} of either block, then 64 B of scales, i's
+//         {tokens 2i, 2i+1} of either block
 //   Q4_0: per block and k-step (k 8i + 4 step ..) 512 B, the lane's {hi, hi, lo, lo}
 // ---------------------------------------------------------------------------
 template <int QT>
-constexpr int xgroup_bytes() { return QT == PI_QT_Q8_0 ? 2 * 512 + 2 * 64 : 8 * 512; }
+constexpr int xunit_bytes() { return QT == PI_QT_Q8_0 ? 512 + 64 : 4 * 512; }
+
+PI_DEV uint32_t to_tf32(float v) {
+    uint32_t r;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(v));
+    return r;
+}
 
 // Within a chunk the columns are ordered by adapter, those without one first, so that an
 // n-tile holds few adapters: the column of a token is the number of tokens of its chunk
@@ -168,7 +173,7 @@ constexpr int PREP_S = 4;   // warps of a unit
 
 template <int QT>
 __global__ __launch_bounds__(PREP_T) void k_proj_prep(const float* __restrict__ x, int64_t T, int64_t n_in,
-                                                      int64_t groups, int NT, uint8_t* __restrict__ xf,
+                                                      int64_t units, int NT, uint8_t* __restrict__ xf,
                                                       float* __restrict__ xs, const LoraArgs L,
                                                       float* __restrict__ h, uint32_t* err) {
     pdl_wait();
@@ -191,15 +196,15 @@ __global__ __launch_bounds__(PREP_T) void k_proj_prep(const float* __restrict__ 
         }
         const int g = col & 7;
         const float* xr = x + t * n_in;
-        uint8_t* xo = xf + (chunk * groups * NT + (col >> 3)) * xgroup_bytes<QT>();
-        const int64_t gstride = (int64_t)NT * xgroup_bytes<QT>();
+        uint8_t* xo = xf + (chunk * units * NT + (col >> 3)) * xunit_bytes<QT>();
+        const int64_t ustride = (int64_t)NT * xunit_bytes<QT>();
         if (L.ids && tid == 0) {
             const int a = L.ids[t];
             if (a >= L.n) atomicOr(err, PI_DEVERR_INDEX);
         }
         if constexpr (QT == PI_QT_Q8_0) {
-            for (int64_t c = warp; c < groups; c += PREP_T / 32) {
-                const int64_t k = c * 128 + lane * 4;
+            for (int64_t c = warp; 2 * c < units; c += PREP_T / 32) {  // four blocks
+                const int64_t k = c * 128 + lane * 4, u = 2 * c + (lane >> 4);
                 float e[4] = {0.f, 0.f, 0.f, 0.f};
                 if (k < n_in) {
                     const float4 v = *reinterpret_cast<const float4*>(xr + k);
@@ -207,11 +212,11 @@ __global__ __launch_bounds__(PREP_T) void k_proj_prep(const float* __restrict__ 
                 }
                 float sc;
                 const uint32_t q = quad_quant_q8(e, &sc);
-                const int b = lane >> 3, j = lane & 7;  // eighth j of the group's block b
-                uint8_t* o = xo + c * gstride;
-                *reinterpret_cast<uint32_t*>(o + (b >> 1) * 512 + (g * 4 + (j & 3)) * 16 + (b & 1) * 8 + (j >> 2) * 4) = q;
-                if (j == 0)
-                    *reinterpret_cast<float*>(o + 1024 + (b >> 1) * 64 + (g >> 1) * 16 + (b & 1) * 8 + (g & 1) * 4) = sc;
+                if (u >= units) continue;
+                const int b = (lane >> 3) & 1, j = lane & 7;  // eighth j of the unit's block b
+                uint8_t* o = xo + u * ustride;
+                *reinterpret_cast<uint32_t*>(o + (g * 4 + (j & 3)) * 16 + b * 8 + (j >> 2) * 4) = q;
+                if (j == 0) *reinterpret_cast<float*>(o + 512 + (g >> 1) * 16 + b * 8 + (g & 1) * 4) = sc;
             }
         } else {
             __shared__ float s_m[PREP_T / 32];
@@ -231,7 +236,7 @@ __global__ __launch_bounds__(PREP_T) void k_proj_prep(const float* __restrict__ 
             const bool fin = m < INFINITY;
             const float s = fin ? ldexpf(1.0f, ex) : __int_as_float(0x7fffffff);
             if (tid == 0) xs[t] = fin ? ldexpf(1.0f, -ex) : __int_as_float(0x7fffffff);
-            for (int64_t j = tid; j < groups * 16; j += PREP_T) {  // eight values: lane i = j % 4 of block j / 4
+            for (int64_t j = tid; j < units * 8; j += PREP_T) {  // eight values: lane i = j % 4 of block j / 4
                 float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
                 if (j * 8 < n_in) {
                     const float4 u = *reinterpret_cast<const float4*>(xr + j * 8);
@@ -248,14 +253,15 @@ __global__ __launch_bounds__(PREP_T) void k_proj_prep(const float* __restrict__ 
                     hi[p] = *reinterpret_cast<const uint32_t*>(&a);
                     lo[p] = *reinterpret_cast<const uint32_t*>(&c);
                 }
-                uint8_t* o = xo + (j >> 4) * gstride + ((j >> 2) & 3) * 1024 + (g * 4 + (j & 3)) * 16;
+                uint8_t* o = xo + (j >> 3) * ustride + ((j >> 2) & 1) * 1024 + (g * 4 + (j & 3)) * 16;
                 *reinterpret_cast<uint4*>(o) = make_uint4(hi[0], hi[1], lo[0], lo[1]);
                 *reinterpret_cast<uint4*>(o + 512) = make_uint4(hi[2], hi[3], lo[2], lo[3]);
             }
         }
         return;
     }
-    // h[t][r] = scale * (A[a][r] . x[t])
+    // h[t][r] = scale * (A[a][r] . x[t]), zero from the rank on, as two tf32 terms: per unit
+    // of four rank rows the four large terms, then the four small ones
     __shared__ float s_h[PREP_T / 32][PREP_R];
     const int per = L.R / PREP_R, part = warp % PREP_S;
     const int64_t unit = (blockIdx.x - T) * (PREP_T / 32 / PREP_S) + warp / PREP_S, t = unit / per;
@@ -296,7 +302,11 @@ __global__ __launch_bounds__(PREP_T) void k_proj_prep(const float* __restrict__ 
         float s = 0.0f;
 #pragma unroll
         for (int q = 0; q < PREP_S; ++q) s += s_h[warp + q][lane];
-        h[t * L.R + r0 + lane] = s * (L.scales ? L.scales[a] : 1.0f);
+        s = r0 + lane < rank ? s * (L.scales ? L.scales[a] : 1.0f) : 0.0f;
+        const uint32_t big = to_tf32(s);
+        float* o = h + (t * L.R + r0) * 2 + lane;
+        o[0] = __uint_as_float(big);
+        o[PREP_R] = __uint_as_float(to_tf32(s - __uint_as_float(big)));
     }
 }
 
@@ -310,21 +320,16 @@ struct ProjArgs {
     const float* h;
     float* y;
     LoraArgs L;
-    int64_t T, n_out, groups, tiles;
+    int64_t T, n_out, units, tiles;
     int ks;      // CTAs that share the blocks of their rows
-    int cg;      // groups of a part that are staged together
+    int cu;      // units of a part that are staged together
     int nchunk;  // such pieces of a part
 };
-
-// 1.5 * 2^23 as bits: an integer sum below 2^22 added to these bits is the float
-// 1.5 * 2^23 + sum, so accumulating on it replaces the conversion by one subtraction.
-constexpr int FLOAT_BIAS_BITS = 0x4B400000;
-constexpr float FLOAT_BIAS = 12582912.0f;
 
 PI_DEV void mma_s8(int (&c)[4], const uint4& a, const uint2& b) {
     asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
         : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
-        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(FLOAT_BIAS_BITS));
+        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(0));
 }
 PI_DEV void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -339,16 +344,18 @@ PI_DEV uint32_t nib_pair(uint32_t w, int p) {
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// A lane's words of one group of a tile.
+// A lane's words of one unit of a tile.
 template <int QT>
-struct GroupRegs {
-    static constexpr int NQ = QT == PI_QT_Q8_0 ? 4 : 2;
+struct UnitRegs {
+    static constexpr int NQ = QT == PI_QT_Q8_0 ? 2 : 1;
     int4 q[NQ];
-    int4 d;
+    int2 d;
     PI_DEV void load(const uint8_t* p, int lane) {
 #pragma unroll
         for (int i = 0; i < NQ; ++i) q[i] = ld_stream(p + i * 512 + lane * 16);
-        d = ld_stream(p + NQ * 512 + (lane >> 2) * 16);
+        asm volatile("ld.global.nc.L1::no_allocate.v2.s32 {%0,%1}, [%2];"
+                     : "=r"(d.x), "=r"(d.y)
+                     : "l"(p + NQ * 512 + (lane >> 2) * 8));
     }
 };
 PI_DEV int word(const int4& v, int i) { return i == 0 ? v.x : (i == 1 ? v.y : (i == 2 ? v.z : v.w)); }
@@ -358,11 +365,6 @@ PI_DEV void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-PI_DEV uint32_t to_tf32(float v) {
-    uint32_t r;
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(v));
-    return r;
-}
 
 PI_DEV void cp_async16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -370,14 +372,15 @@ PI_DEV void cp_async16(uint32_t dst, const void* src) {
 
 constexpr int GEMM_T = 256;
 constexpr int GEMM_W = GEMM_T / 32;
+constexpr int RING = 4;  // units a warp holds or has in flight (4 KB of Q8_0 weights)
 
 // CTA = 8 warps of 16 rows each; blockIdx.x = the CTA's part of the blocks (the ks CTAs of a
-// cluster share their rows) + ks * the set of 128 rows; blockIdx.y: the chunk of NT n-tiles.
-// The weights stream from memory once per chunk straight into registers, the next group's
-// 16-byte loads in flight while the current one is multiplied; the activations' fragments
-// come through a stage in shared memory that the CTA's warps share, double-buffered where a
-// part does not fit. Splitting over CTAs rather than over a CTA's warps keeps 128 rows to
-// every staged fragment (n_out 12288, T 16, Q4_0: 54 us with the blocks split over the warps).
+// cluster share their rows) + ks * the set of 128 rows; blockIdx.y: the chunk of NT
+// n-tiles. The weights stream from memory once per chunk straight into a ring of D units in
+// registers; the activations' fragments come through a stage in shared memory that the
+// CTA's warps share, double-buffered where a part does not fit. Splitting over CTAs rather
+// than over a CTA's warps keeps 128 rows to every staged fragment (n_out 12288, T 16, Q4_0:
+// 54 us with the blocks split over the warps, 36 over a cluster).
 //
 // Adapters: for every (adapter, n-tile) that meet, one product of the adapter's rows of B
 // (exact in tf32 for f16 and bf16 weights, two tf32 terms for f32 ones) with h in two tf32
@@ -385,31 +388,35 @@ constexpr int GEMM_W = GEMM_T / 32;
 // an adapter's NaN stays with its requests.
 template <int QT, int NT>
 __global__ __launch_bounds__(GEMM_T, 2) void k_proj_gemm(const ProjArgs p) {
-    constexpr int XG = xgroup_bytes<QT>(), GB = group_bytes<QT>(), NC = 8 * NT;
-    extern __shared__ __align__(16) uint8_t s_x[];  // [2][cg][NT] fragment groups, then the sums
+    constexpr int XU = xunit_bytes<QT>(), UB = unit_bytes<QT>(), NC = 8 * NT, D = RING;
+    extern __shared__ __align__(16) uint8_t s_x[];  // [2][cu][NT] fragment units, then the sums
     __shared__ int s_key[NC], s_id[NC], s_rank[NC], s_tok[NC], s_pair[NC], s_npair;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, i4 = lane & 3;
     const int ks = p.ks, part = (int)(blockIdx.x % ks);
     const int64_t tile = (int64_t)(blockIdx.x / ks) * GEMM_W + warp;
     const int64_t t0 = (int64_t)blockIdx.y * NC;
     const int ncol = (int)min((int64_t)NC, p.T - t0);
-    const int64_t gb = p.groups * part / ks, ge = p.groups * (part + 1) / ks;
+    const int ub = (int)(p.units * part / ks), ue = (int)(p.units * (part + 1) / ks);
     const bool live = tile < p.tiles;
-    const uint8_t* wt = p.w + tile * p.groups * GB;
-    GroupRegs<QT> ra, rb;
-    if (live && gb < ge) ra.load(wt + gb * GB, lane);  // constant weights: before the wait
+    const uint8_t* wt = p.w + tile * p.units * UB;
+    UnitRegs<QT> ring[D];
+    if (live) {
+#pragma unroll
+        for (int d = 0; d < D; ++d)  // constant weights: before the wait
+            if (ub + d < ue) ring[d].load(wt + (int64_t)(ub + d) * UB, lane);
+    }
     pdl_wait();
     pdl_trigger();
 
-    const uint8_t* xsrc = p.xf + (int64_t)blockIdx.y * p.groups * (NT * XG);
+    const uint8_t* xsrc = p.xf + (int64_t)blockIdx.y * p.units * (NT * XU);
     const uint32_t s_base = (uint32_t)__cvta_generic_to_shared(s_x);
-    const int stage_bytes = p.cg * (NT * XG);
+    const int stage_bytes = p.cu * (NT * XU);
     auto stage = [&](int c) {
-        const int64_t b = gb + (int64_t)c * p.cg, e = min(ge, b + p.cg);
-        const int n16 = (int)(max((int64_t)0, e - b) * (NT * XG / 16));
+        const int b = ub + c * p.cu, e = min(ue, b + p.cu);
+        const int n16 = max(0, e - b) * (NT * XU / 16);
         const uint32_t dst = s_base + (c & 1) * stage_bytes;
-        const uint8_t* src = xsrc + b * (NT * XG);
-        for (int i = tid; i < n16; i += GEMM_T) cp_async16(dst + i * 16, src + i * 16);
+        const uint8_t* src = xsrc + (int64_t)b * (NT * XU);
+        for (int i = tid; i < n16; i += GEMM_T) cp_async16(dst + i * 16, src + (int64_t)i * 16);
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     stage(0);
@@ -449,59 +456,54 @@ __global__ __launch_bounds__(GEMM_T, 2) void k_proj_gemm(const ProjArgs p) {
     uint64_t sum[NT][2];  // pairs of neighbouring columns, rows g and g + 8
 #pragma unroll
     for (int n = 0; n < NT; ++n) sum[n][0] = sum[n][1] = 0;
-    auto multiply = [&](const GroupRegs<QT>& w, const uint8_t* xg) {
+    auto multiply = [&](const UnitRegs<QT>& w, const uint8_t* xu) {
+        uint64_t dg[2][2];  // [block]{d, d} of rows g and g + 8
 #pragma unroll
-        for (int hb = 0; hb < 2; ++hb) {  // two blocks at a time
-            uint64_t dg[2][2];            // [block]{d, d} of rows g and g + 8
+        for (int b = 0; b < 2; ++b) {
+            const int v = b ? w.d.y : w.d.x;
+            const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&v));
+            dg[b][0] = pack2(d.x, d.x);
+            dg[b][1] = pack2(d.y, d.y);
+        }
+        if constexpr (QT == PI_QT_Q8_0) {
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const int v = word(w.d, 2 * hb + b);
-                const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&v));
-                dg[b][0] = pack2(d.x, d.x);
-                dg[b][1] = pack2(d.y, d.y);
-            }
-            if constexpr (QT == PI_QT_Q8_0) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const uint4 xv = *reinterpret_cast<const uint4*>(xg + n * XG + hb * 512 + lane * 16);
-                    const ulonglong2 dx = *reinterpret_cast<const ulonglong2*>(xg + n * XG + 1024 + hb * 64 + i4 * 16);
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        int s[4];
-                        mma_s8(s, *reinterpret_cast<const uint4*>(&w.q[2 * hb + b]),
-                               b ? make_uint2(xv.z, xv.w) : make_uint2(xv.x, xv.y));
-                        const uint64_t bias = pack2(-FLOAT_BIAS, -FLOAT_BIAS), d2 = b ? dx.y : dx.x;
-                        const uint64_t f0 = add2(pack2(__int_as_float(s[0]), __int_as_float(s[1])), bias);
-                        const uint64_t f1 = add2(pack2(__int_as_float(s[2]), __int_as_float(s[3])), bias);
-                        sum[n][0] = fma2(f0, mul2(dg[b][0], d2), sum[n][0]);
-                        sum[n][1] = fma2(f1, mul2(dg[b][1], d2), sum[n][1]);
-                    }
-                }
-            } else {
+            for (int n = 0; n < NT; ++n) {
+                const uint4 xv = *reinterpret_cast<const uint4*>(xu + n * XU + lane * 16);
+                const ulonglong2 dx = *reinterpret_cast<const ulonglong2*>(xu + n * XU + 512 + i4 * 16);
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
-                    uint32_t a[2][4];
-                    const uint32_t w0 = word(w.q[hb], 2 * b), w1 = word(w.q[hb], 2 * b + 1);
+                    int s[4];
+                    mma_s8(s, *reinterpret_cast<const uint4*>(&w.q[b]),
+                           b ? make_uint2(xv.z, xv.w) : make_uint2(xv.x, xv.y));
+                    const uint64_t d2 = b ? dx.y : dx.x;
+                    sum[n][0] = fma2(pack2((float)s[0], (float)s[1]), mul2(dg[b][0], d2), sum[n][0]);
+                    sum[n][1] = fma2(pack2((float)s[2], (float)s[3]), mul2(dg[b][1], d2), sum[n][1]);
+                }
+            }
+        } else {
 #pragma unroll
-                    for (int s = 0; s < 2; ++s) {
-                        a[s][0] = nib_pair(w0, 2 * s);
-                        a[s][1] = nib_pair(w1, 2 * s);
-                        a[s][2] = nib_pair(w0, 2 * s + 1);
-                        a[s][3] = nib_pair(w1, 2 * s + 1);
-                    }
+            for (int b = 0; b < 2; ++b) {
+                uint32_t a[2][4];
+                const uint32_t w0 = word(w.q[0], 2 * b), w1 = word(w.q[0], 2 * b + 1);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        const uint8_t* xb = xg + n * XG + (2 * hb + b) * 1024 + lane * 16;
-                        const uint4 x0 = *reinterpret_cast<const uint4*>(xb);
-                        const uint4 x1 = *reinterpret_cast<const uint4*>(xb + 512);
-                        float s[4] = {0.f, 0.f, 0.f, 0.f};
-                        mma_f16(s, a[0], x0.z, x0.w);
-                        mma_f16(s, a[1], x1.z, x1.w);
-                        mma_f16(s, a[0], x0.x, x0.y);
-                        mma_f16(s, a[1], x1.x, x1.y);
-                        sum[n][0] = fma2(dg[b][0], pack2(s[0], s[1]), sum[n][0]);
-                        sum[n][1] = fma2(dg[b][1], pack2(s[2], s[3]), sum[n][1]);
-                    }
+                for (int s = 0; s < 2; ++s) {
+                    a[s][0] = nib_pair(w0, 2 * s);
+                    a[s][1] = nib_pair(w1, 2 * s);
+                    a[s][2] = nib_pair(w0, 2 * s + 1);
+                    a[s][3] = nib_pair(w1, 2 * s + 1);
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const uint8_t* xb = xu + n * XU + b * 1024 + lane * 16;
+                    const uint4 x0 = *reinterpret_cast<const uint4*>(xb);
+                    const uint4 x1 = *reinterpret_cast<const uint4*>(xb + 512);
+                    float s[4] = {0.f, 0.f, 0.f, 0.f};
+                    mma_f16(s, a[0], x0.z, x0.w);
+                    mma_f16(s, a[1], x1.z, x1.w);
+                    mma_f16(s, a[0], x0.x, x0.y);
+                    mma_f16(s, a[1], x1.x, x1.y);
+                    sum[n][0] = fma2(dg[b][0], pack2(s[0], s[1]), sum[n][0]);
+                    sum[n][1] = fma2(dg[b][1], pack2(s[2], s[3]), sum[n][1]);
                 }
             }
         }
@@ -511,16 +513,17 @@ __global__ __launch_bounds__(GEMM_T, 2) void k_proj_gemm(const ProjArgs p) {
         __syncthreads();  // piece c has landed; nobody reads the other buffer any more
         if (c + 1 < p.nchunk) stage(c + 1);
         if (!live) continue;
-        const uint8_t* xg = s_x + (c & 1) * stage_bytes;
-        const int64_t g0 = gb + (int64_t)c * p.cg, g1 = min(ge, g0 + p.cg);
-        // two register sets in turn; a piece that is not the last has an even number of groups
+        const uint8_t* xu = s_x + (c & 1) * stage_bytes;
+        const int u0 = ub + c * p.cu, u1 = min(ue, u0 + p.cu);
+        // a piece that is not the last has a multiple of D units, so unit u0 is in ring[0]
 #pragma unroll 1
-        for (int64_t gr = g0; gr < g1; gr += 2, xg += 2 * NT * XG) {
-            if (gr + 1 < ge) rb.load(wt + (gr + 1) * GB, lane);
-            multiply(ra, xg);
-            if (gr + 1 >= g1) break;
-            if (gr + 2 < ge) ra.load(wt + (gr + 2) * GB, lane);
-            multiply(rb, xg + NT * XG);
+        for (int u = u0; u < u1; u += D, xu += D * NT * XU) {
+#pragma unroll
+            for (int d = 0; d < D; ++d) {
+                if (u + d >= u1) break;
+                multiply(ring[d], xu + d * NT * XU);
+                if (u + d + D < ue) ring[d].load(wt + (int64_t)(u + d + D) * UB, lane);
+            }
         }
     }
     float acc[NT][4];
@@ -546,8 +549,8 @@ __global__ __launch_bounds__(GEMM_T, 2) void k_proj_gemm(const ProjArgs p) {
             if (n % ks != part) continue;
             float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
             for (int q = 0; q < ks; ++q) {
-                const float4 v =
-                    *reinterpret_cast<const float4*>(cl.map_shared_rank(sums, q) + ((warp * NT + n) * 32 + lane) * 4);
+                const float4 v = *reinterpret_cast<const float4*>(cl.map_shared_rank(sums, q) +
+                                                                  ((warp * NT + n) * 32 + lane) * 4);
                 t.x += v.x;
                 t.y += v.y;
                 t.z += v.z;
@@ -574,85 +577,96 @@ __global__ __launch_bounds__(GEMM_T, 2) void k_proj_gemm(const ProjArgs p) {
     }
     const int npair = s_npair;
     if (npair) {
+        const bool f32 = p.L.dtype == PI_QT_F32, f16 = p.L.dtype == PI_QT_F16;
+        const int es = f32 ? 4 : 2;
+        const uint8_t* bt = reinterpret_cast<const uint8_t*>(p.L.b) + (tile * 16 + g) * p.L.R * es;
+        const int64_t per_adapter = p.n_out * p.L.R * es, eight = (int64_t)8 * p.L.R * es;
         struct Item {
-            uint4 b[2];  // four rank entries of rows g and g + 8 as they are stored
-            float4 h;
+            uint4 b[2];   // four rank entries of rows g and g + 8 as they are stored
+            float4 h[2];  // h of the lane's column, large and small terms
         } cur, nxt;
         auto fetch = [&](Item& it, int i, int r0) {
-            const int j = s_pair[i], a = s_id[j], r = r0 + 4 * i4;
+            const int j = s_pair[i], a = s_id[j], r = r0 + 4 * i4, col = (j & ~7) + g;
             const bool in = r < s_rank[j];
+            const uint8_t* bp = bt + a * per_adapter + r * es;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const int64_t row = tile * 16 + g + 8 * k, off = ((int64_t)a * p.n_out + row) * p.L.R + r;
                 it.b[k] = make_uint4(0, 0, 0, 0);
-                if (in && row < p.n_out) {
-                    if (p.L.dtype == PI_QT_F32) {
-                        it.b[k] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(p.L.b) + off));
+                if (in && (tile * 16 + g) + 8 * k < p.n_out) {
+                    if (f32) {
+                        it.b[k] = __ldg(reinterpret_cast<const uint4*>(bp + k * eight));
                     } else {
-                        const uint2 v = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p.L.b) + off));
+                        const uint2 v = __ldg(reinterpret_cast<const uint2*>(bp + k * eight));
                         it.b[k].x = v.x;
                         it.b[k].y = v.y;
                     }
                 }
             }
-            const int col = (j & ~7) + g;
-            it.h = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (in && s_id[col] == a) it.h = *reinterpret_cast<const float4*>(p.h + (t0 + s_tok[col]) * p.L.R + r);
+            it.h[0] = it.h[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (in && s_id[col] == a) {
+                const float4* hp = reinterpret_cast<const float4*>(p.h + ((t0 + s_tok[col]) * p.L.R + r) * 2);
+                it.h[0] = hp[0];
+                it.h[1] = hp[1];
+            }
         };
         float c[4] = {0.f, 0.f, 0.f, 0.f};
         int i = 0, r0 = 0;
         fetch(cur, 0, 0);
         while (i < npair) {
-            const int j = s_pair[i], rank = s_rank[j], a = s_id[j];
+            const int j = s_pair[i], rank = s_rank[j];
             const bool last = r0 + 16 >= rank;
             const int ni = last ? i + 1 : i, nr = last ? 0 : r0 + 16;
             if (ni < npair) fetch(nxt, ni, nr);
             const int left = rank - r0 - 4 * i4;  // rank entries of this lane's four that count
-            float bv[2][4];
+            const uint32_t* hb = reinterpret_cast<const uint32_t*>(&cur.h[0]);
+            const uint32_t* hs = reinterpret_cast<const uint32_t*>(&cur.h[1]);
+            uint32_t big[2][4], small[2][4];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const uint4 v = cur.b[k];
-                if (p.L.dtype == PI_QT_F32) {
-                    bv[k][0] = __uint_as_float(v.x);
-                    bv[k][1] = __uint_as_float(v.y);
-                    bv[k][2] = __uint_as_float(v.z);
-                    bv[k][3] = __uint_as_float(v.w);
-                } else if (p.L.dtype == PI_QT_F16) {
+                float f[4];
+                if (f32) {
+                    f[0] = __uint_as_float(v.x);
+                    f[1] = __uint_as_float(v.y);
+                    f[2] = __uint_as_float(v.z);
+                    f[3] = __uint_as_float(v.w);
+                } else if (f16) {
                     const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&v.x));
                     const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
-                    bv[k][0] = x.x;
-                    bv[k][1] = x.y;
-                    bv[k][2] = y.x;
-                    bv[k][3] = y.y;
+                    f[0] = x.x;
+                    f[1] = x.y;
+                    f[2] = y.x;
+                    f[3] = y.y;
                 } else {
-                    bv[k][0] = __uint_as_float(v.x << 16);
-                    bv[k][1] = __uint_as_float(v.x & 0xffff0000u);
-                    bv[k][2] = __uint_as_float(v.y << 16);
-                    bv[k][3] = __uint_as_float(v.y & 0xffff0000u);
+                    f[0] = __uint_as_float(v.x << 16);
+                    f[1] = __uint_as_float(v.x & 0xffff0000u);
+                    f[2] = __uint_as_float(v.y << 16);
+                    f[3] = __uint_as_float(v.y & 0xffff0000u);
                 }
-            }
-            const float hv[4] = {cur.h.x, cur.h.y, cur.h.z, cur.h.w};
-            uint32_t big[2][4], small[2][4], hb[4], hs[4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const float h = q < left ? hv[q] : 0.0f;
-                hb[q] = to_tf32(h);
-                hs[q] = to_tf32(h - __uint_as_float(hb[q]));
+                for (int q = 1; q < 4; ++q)
+                    if (q >= left) f[q] = 0.0f;  // entry 0 past the rank was not loaded
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const float f = q < left ? bv[k][q] : 0.0f;
-                    big[q >> 1][k + 2 * (q & 1)] = to_tf32(f);
-                    small[q >> 1][k + 2 * (q & 1)] = to_tf32(f - __uint_as_float(to_tf32(f)));
-                }
+                for (int q = 0; q < 4; ++q) big[q >> 1][k + 2 * (q & 1)] = __float_as_uint(f[q]);
             }
+            if (f32) {
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                if (p.L.dtype == PI_QT_F32) mma_tf32(c, small[s], hb[2 * s], hb[2 * s + 1]);
-                mma_tf32(c, big[s], hs[2 * s], hs[2 * s + 1]);
-                mma_tf32(c, big[s], hb[2 * s], hb[2 * s + 1]);
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const float f = __uint_as_float(big[s][q]);
+                        big[s][q] = to_tf32(f);
+                        small[s][q] = to_tf32(f - __uint_as_float(big[s][q]));
+                    }
+                mma_tf32(c, small[0], hb[0], hb[1]);
+                mma_tf32(c, small[1], hb[2], hb[3]);
             }
+            mma_tf32(c, big[0], hs[0], hs[1]);
+            mma_tf32(c, big[1], hs[2], hs[3]);
+            mma_tf32(c, big[0], hb[0], hb[1]);
+            mma_tf32(c, big[1], hb[2], hb[3]);
             if (last) {
-                const int n0 = j >> 3;
+                const int n0 = j >> 3, a = s_id[j];
                 const bool u0 = s_id[n0 * 8 + 2 * i4] == a, u1 = s_id[n0 * 8 + 2 * i4 + 1] == a;
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
@@ -707,17 +721,17 @@ ProjBufs proj_carve(const pi_proj* P, int64_t T, int64_t R, char* base) {
     PiBump b{base};
     ProjBufs o;
     const int64_t NT = proj_chunk(T), chunks = ((T + 7) / 8 + NT - 1) / NT;
-    const int64_t xg = P->qtype == PI_QT_Q8_0 ? xgroup_bytes<PI_QT_Q8_0>() : xgroup_bytes<PI_QT_Q4_0>();
-    o.xf = b.take<uint8_t>((size_t)(chunks * P->groups * NT * xg));
+    const int64_t xg = P->qtype == PI_QT_Q8_0 ? xunit_bytes<PI_QT_Q8_0>() : xunit_bytes<PI_QT_Q4_0>();
+    o.xf = b.take<uint8_t>((size_t)(chunks * P->units * NT * xg));
     o.xs = b.take<float>((size_t)(P->qtype == PI_QT_Q4_0 ? T : 0));
-    o.h = b.take<float>((size_t)(T * R));
+    o.h = b.take<float>((size_t)(T * R) * 2);
     o.bytes = b.off + 256;
     return o;
 }
 
 template <int QT>
 int proj_pack(pi_ctx* ctx, pi_proj* P, const uint8_t* raw, int src_on_host) {
-    const int64_t nb = P->n_in / 32, row_bytes = proj_raw_bytes(QT, P->n_in), stride = P->groups * group_bytes<QT>();
+    const int64_t nb = P->n_in / 32, row_bytes = proj_raw_bytes(QT, P->n_in), stride = P->units * unit_bytes<QT>();
     // a host source comes over in runs of whole tiles, 64 MB at most
     const int64_t per = src_on_host ? std::max<int64_t>(1, (64 << 20) / (16 * row_bytes)) : P->tiles;
     uint8_t* stage = nullptr;
@@ -734,7 +748,7 @@ int proj_pack(pi_ctx* ctx, pi_proj* P, const uint8_t* raw, int src_on_host) {
             src = stage;
         }
         if (rc) break;
-        k_proj_pack<QT><<<(unsigned)(nt * P->groups), 128>>>(src, nb, rows, P->groups, P->w + t * stride);
+        k_proj_pack<QT><<<(unsigned)(nt * P->units), 64>>>(src, nb, rows, P->units, P->w + t * stride);
         if (pi_cuda_check(ctx, cudaDeviceSynchronize(), "projection pack")) rc = PI_ERR_CUDA;
     }
     if (stage) cudaFree(stage);
@@ -758,15 +772,15 @@ int proj_create(pi_ctx* ctx, const void* raw, uint64_t raw_len, int32_t qtype, i
     P->qtype = qtype;
     P->n_in = n_in;
     P->n_out = n_out;
-    P->groups = (n_in / 32 + 3) / 4;
+    P->units = (n_in / 32 + 1) / 2;
     P->tiles = (n_out + 15) / 16;
-    const int64_t gbytes = qtype == PI_QT_Q8_0 ? group_bytes<PI_QT_Q8_0>() : group_bytes<PI_QT_Q4_0>();
-    if (P->tiles * P->groups > INT32_MAX) {
+    const int64_t ubytes = qtype == PI_QT_Q8_0 ? unit_bytes<PI_QT_Q8_0>() : unit_bytes<PI_QT_Q4_0>();
+    if (P->tiles * P->units > INT32_MAX) {
         delete P;
         return pi_set_error(ctx, PI_ERR_ARG, "projection: too large");
     }
     int rc = PI_OK;
-    if (pi_cuda_check(ctx, cudaMalloc((void**)&P->w, (size_t)(P->tiles * P->groups * gbytes)), "cudaMalloc(projection)"))
+    if (pi_cuda_check(ctx, cudaMalloc((void**)&P->w, (size_t)(P->tiles * P->units * ubytes)), "cudaMalloc(projection)"))
         rc = PI_ERR_OOM;
     if (!rc)
         rc = qtype == PI_QT_Q8_0 ? proj_pack<PI_QT_Q8_0>(ctx, P, (const uint8_t*)raw, src_on_host)
@@ -781,28 +795,28 @@ int proj_create(pi_ctx* ctx, const void* raw, uint64_t raw_len, int32_t qtype, i
 
 template <int QT, int NT>
 cudaError_t launch_gemm(ProjArgs a, int64_t sms, cudaStream_t st) {
-    constexpr int XG = NT * xgroup_bytes<QT>();
-    const int64_t sets = (a.tiles + GEMM_W - 1) / GEMM_W, chunks = ((a.T + 8 * NT - 1) / (8 * NT));
-    // Parts of the blocks: the time is about the rounds of CTAs, two to an SM, times the groups
-    // of a part plus what a CTA costs beside them (start, stage and join, about six groups)
+    constexpr int XU = NT * xunit_bytes<QT>(), D = RING;
+    const int64_t sets = (a.tiles + GEMM_W - 1) / GEMM_W, chunks = (a.T + 8 * NT - 1) / (8 * NT);
+    // Parts of the blocks: the time is about the rounds of CTAs, two to an SM, times the units
+    // of a part plus what a CTA costs beside them (start, stage and join, about a dozen units)
     a.ks = 1;
     int64_t best = INT64_MAX;
-    for (int ks = 1; ks <= 8 && ks <= a.groups; ++ks) {
+    for (int ks = 1; ks <= 8 && ks <= a.units; ++ks) {
         const int64_t rounds = (sets * chunks * ks + 2 * sms - 1) / (2 * sms);
-        const int64_t cost = rounds * ((a.groups + ks - 1) / ks + 6);
+        const int64_t cost = rounds * ((a.units + ks - 1) / ks + 12);
         if (cost < best) {
             best = cost;
             a.ks = ks;
         }
     }
-    // A part is staged whole where two CTAs of an SM have room for it, in pieces of an even
-    // number of groups otherwise
-    const int64_t budget = 100 * 1024, part = (a.groups + a.ks - 1) / a.ks;
-    a.cg = (int)part;
-    if (part * XG > budget) a.cg = (int)std::max<int64_t>(2, budget / 2 / XG / 2 * 2);
-    a.nchunk = (int)((part + a.cg - 1) / a.cg);
+    // A part is staged whole where two CTAs of an SM have room for it, in pieces of a multiple
+    // of D units otherwise
+    const int64_t budget = 100 * 1024, part = (a.units + a.ks - 1) / a.ks;
+    a.cu = (int)part;
+    if (part * XU > budget) a.cu = (int)std::max<int64_t>(D, budget / 2 / XU / D * D);
+    a.nchunk = (int)((part + a.cu - 1) / a.cu);
     const size_t sums = a.ks > 1 ? (size_t)GEMM_W * NT * 512 : 0;
-    const size_t smem = std::max<size_t>((size_t)std::min(a.nchunk, 2) * a.cg * XG, sums);
+    const size_t smem = std::max<size_t>((size_t)std::min(a.nchunk, 2) * a.cu * XU, sums);
     auto kern = k_proj_gemm<QT, NT>;
     pi_smem_attr((const void*)kern, smem);
     cudaLaunchConfig_t cfg = {};
@@ -872,15 +886,15 @@ int proj_forward(pi_ctx* ctx, const pi_proj* P, const float* x, int64_t T, const
         PiProfScope ps(ctx, st, "k_proj_prep");
         const int64_t units = T * (R / PREP_R), per = PREP_T / 32 / PREP_S, grid = T + (units + per - 1) / per;
         if (q8)
-            pi_pdl_launch(k_proj_prep<PI_QT_Q8_0>, dim3((unsigned)grid), dim3(PREP_T), 0, st, x, T, P->n_in, P->groups,
+            pi_pdl_launch(k_proj_prep<PI_QT_Q8_0>, dim3((unsigned)grid), dim3(PREP_T), 0, st, x, T, P->n_in, P->units,
                           NT, B.xf, B.xs, L, B.h, ctx->dev_err);
         else
-            pi_pdl_launch(k_proj_prep<PI_QT_Q4_0>, dim3((unsigned)grid), dim3(PREP_T), 0, st, x, T, P->n_in, P->groups,
+            pi_pdl_launch(k_proj_prep<PI_QT_Q4_0>, dim3((unsigned)grid), dim3(PREP_T), 0, st, x, T, P->n_in, P->units,
                           NT, B.xf, B.xs, L, B.h, ctx->dev_err);
     }
     {
         PiProfScope ps(ctx, st, "k_proj_gemm");
-        const ProjArgs a{P->w, B.xf, B.xs, B.h, y, L, T, P->n_out, P->groups, P->tiles, 1, 1, 1};
+        const ProjArgs a{P->w, B.xf, B.xs, B.h, y, L, T, P->n_out, P->units, P->tiles, 1, 1, 1};
         const int64_t sms = ctx->sm_count > 0 ? ctx->sm_count : 148;
         const cudaError_t e = q8 ? dispatch_gemm<PI_QT_Q8_0>(a, NT, sms, st) : dispatch_gemm<PI_QT_Q4_0>(a, NT, sms, st);
         if (e != cudaSuccess) return pi_cuda_check(ctx, e, "projection");

@@ -98,10 +98,14 @@ class MoeLayer:
         """MoE FFN of tokens x [T, d] (device f32) -> out [T, d].
 
         path: "auto" (tensor-core GEMM for prefill-sized Q4_0 batches, else GEMV),
-        "gemv" or "gemm" to force one. fast: the Q8_0 prefill GEMM adds each block
+        "gemv" or "gemm" to force one; "fused": at most 16 tokens of a Q4_0 layer in two
+        kernels (``pi_moe_forward_fused``; the routing of ``route``, sums in another
+        order than "gemv"). fast: the Q8_0 prefill GEMM adds each block
         term with a fused multiply-add (PI_FWD_FAST_SUM; within the parity tolerance,
         not bit-identical).
         """
+        if path == "fused":
+            return self._forward_fused(x, out, rmsnorm, residual, stream, fast)
         torch = _torch()
         xd = quant._f32(x)
         T = xd.numel() // self.n_embd
@@ -113,6 +117,30 @@ class MoeLayer:
         flags |= {"auto": 0, "gemv": PI_FWD_FORCE_GEMV, "gemm": PI_FWD_FORCE_GEMM}[path]
         flags |= PI_FWD_FAST_SUM if fast else 0
         self.ctx.check(lib().pi_moe_forward(self.ctx.h, self.h, ptr(xd), T, ptr(out), flags, stream_ptr(stream)))
+        return out
+
+    def _forward_fused(self, x, out, rmsnorm, residual, stream, fast):
+        torch = _torch()
+        if fast:
+            raise PiError(PI_ERR_ARG, "moe: the fused path has no fast sum")
+        dev = torch.device("cuda", self.ctx.device)
+        x = quant._f32(x)
+        if x.dtype != torch.float32 or x.device != dev or not x.is_contiguous() or x.numel() % self.n_embd:
+            raise PiError(PI_ERR_ARG, f"moe: x must be contiguous f32 [T, {self.n_embd}] on {dev}")
+        T = x.numel() // self.n_embd
+        if out is None:
+            out = torch.empty((T, self.n_embd), dtype=torch.float32, device=dev)
+        elif out.dtype != torch.float32 or out.device != dev or not out.is_contiguous() or \
+                out.numel() != x.numel():
+            raise PiError(PI_ERR_ARG, f"moe: out must be contiguous f32 [T, {self.n_embd}] on {dev}")
+        L, flags = lib(), (PI_FWD_RMSNORM if rmsnorm else 0) | (PI_FWD_RESIDUAL if residual else 0)
+        nbytes = L.pi_moe_fused_workspace(self.h, T)
+        s = torch.cuda.current_stream(dev) if stream is None else stream
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)  # the caching allocator's: one per call and graph
+        if stream is not None:
+            ws.record_stream(s)
+        self.ctx.check(L.pi_moe_forward_fused(self.ctx.h, self.h, x.data_ptr(), T, out.data_ptr(), flags,
+                                              ws.data_ptr() if nbytes else None, nbytes, s.cuda_stream))
         return out
 
     def forward_routed(self, x, out=None, rmsnorm: bool = False, residual: bool = False, stream=None,

@@ -87,7 +87,8 @@ def test_refuses_without_a_gpu():
 @pytest.mark.parametrize("qtype", [8, 2])
 @pytest.mark.parametrize("T,n_in,n_out", [(1, 32, 1), (1, 2048, 2048), (3, 96, 17), (8, 288, 100), (9, 1024, 31),
                                           (16, 4096, 257), (17, 544, 3001), (33, 1024, 1000), (64, 256, 50),
-                                          (65, 160, 333), (130, 512, 77), (5, 64, 40000), (40, 128, 40001)])
+                                          (65, 160, 333), (130, 512, 77), (5, 64, 40000), (40, 128, 40001),
+                                          (18, 96, 80003), (61, 224, 76001), (20, 4096, 40)])
 def test_projection_alone(orc, qtype, T, n_in, n_out):
     import torch
 
@@ -111,7 +112,7 @@ def test_projection_alone(orc, qtype, T, n_in, n_out):
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
 @pytest.mark.parametrize("T,n_in,n_out,n,R", [(1, 2048, 300, 1, 16), (7, 96, 33, 3, 1), (16, 512, 1000, 4, 12),
                                               (37, 1024, 3001, 5, 12), (70, 288, 129, 40, 5), (64, 256, 40000, 6, 8),
-                                              (4, 4096, 64, 2, 64), (12, 320, 200, 3, 130)])
+                                              (4, 4096, 64, 2, 64), (12, 320, 200, 3, 130), (50, 96, 76003, 7, 20)])
 def test_adapters(orc, qtype, dtype, T, n_in, n_out, n, R):
     import torch
 
