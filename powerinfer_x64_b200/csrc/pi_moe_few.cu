@@ -1,20 +1,26 @@
 // The whole MoE layer of a few tokens (at most 16) in two kernels, Q4_0 experts
 // (model/mod.rs:1239-1571; the decode chain of pi_moe.cu takes 7-8 launches):
 //
-//   k_few_logits   RMSNorm (optional) and the router's exact logits
+//   k_few_logits   RMSNorm (optional), the router's logits and a bound of their distance from
+//                  the reference's
 //   k_few_experts  top-k and gates, gate/up and SwiGLU, a barrier of the grid, down, the
 //                  gate-weighted sum, the gated shared expert and the residual
 //
-// Routing keeps the reference's arithmetic bit for bit (sequential f32 logits, its softmax,
-// ties to the lowest index), so the experts and gates are those of pi_moe_route. Expert
-// products are f32 sums of f32 activations and the exact nibble values, one multiply by
-// the block's scale per 32 terms (the reference dequantises and sums sequentially,
+// The experts chosen are the reference's, bit for bit. Its logits are sequential f32 sums
+// (quant/mod.rs:921-935), about 4.2 dependent cycles an input: 5.5 us of a token's 29 at
+// n_embd 2048. Here a logit is summed in 32 segments side by side with a bound of how far
+// the sequential sum can be from it, and a choice that the bounds leave open (0.4% of
+// tokens for normal inputs, and exact ties) is made again from sequential logits and the
+// reference's own softmax and top-k (pi_topk.cuh).
+//
+// Expert products are f32 sums of f32 activations and the exact nibble values, one multiply
+// by the block's scale per 32 terms (the reference dequantises and sums sequentially,
 // quant/mod.rs:958-969): equal to f32 rounding, as on the layer's other Q4_0 paths.
 //
-// Bound: the bytes of the experts that the tokens use, and for one token the latency of the
-// chain: the sequential logit (about 4.2 cycles an input), two launches, the barrier and
-// three dependent trips to memory. k_few_experts is launched cooperatively: its barrier
-// needs every CTA resident, also while another stream runs the same.
+// Bound: the bytes of the experts that the tokens use; for a token or two the latency of the
+// chain (two launches, the barrier and four dependent trips to memory), for many tokens the
+// decoding of nibbles on the integer pipe. k_few_experts is launched cooperatively: its
+// barrier needs every CTA resident, also while another stream runs the same.
 #include "pi_common.cuh"
 #include "pi_internal.h"
 #include "pi_topk.cuh"
@@ -27,99 +33,124 @@ namespace {
 constexpr int FEW_T = 16;  // tokens at most
 
 // ---------------------------------------------------------------------------
-// k_few_logits: CTA = two router rows (row E: the shared expert's gate) and a group of
-// tokens, all in shared memory (row pitch d + 4 floats: a lane's 16-byte reads of its own
-// row fall into distinct banks). Four lanes per token run the reference's four sums of
-// squares, then one lane per (row, token) its sequential logit.
+// k_few_logits: CTA = R router rows (row E: the shared expert's gate) and a group of tokens in
+// shared memory, each row as 32 segments of S = d / 32 floats at a pitch of S + 4 (lanes'
+// 16-byte reads of their own segments then fall into distinct banks). A warp takes a (row,
+// token), lane l its segment l.
+//
+// Distance from the reference (u = 2^-24). A sequential sum rounds each product, u |p_i|, and
+// each partial sum, u |P_i|; the lanes' sums here do no worse, and joining 32 of them adds 5 u
+// sum |p|. With P_start the sum before a lane's segment and L the sum of the absolute partial
+// sums inside it, sum |P_i| <= B = sum over lanes of S |P_start| + L; errors of errors are
+// below d u < 2.5e-4 of that. So |reference - here| <= u (2.2 B + 12 A + 4 (|l| + |bias|)), A =
+// sum |p|, which leaves 3 u A for the normed inputs' own roundings. RMSNorm itself scales
+// all inputs of a token alike: the reference's sum of squares, d / 4 sequential additions
+// in four lanes, moves a logit by at most (d / 8 + 64) u |l|, added with the bias in mind.
 // ---------------------------------------------------------------------------
-constexpr int FL_T = 128, FL_R = 2;
+constexpr int FL_T = 256, FL_W = FL_T / 32;
+constexpr int FL_GROUP = 4;               // tokens of a CTA
+constexpr size_t FL_SMEM = 190 * 1024;
 
 struct FewLogitArgs {
     const float *x, *router, *bias;
-    int T, d, E, group, norm;  // group: tokens of a CTA
-    float *normed, *logits;
+    int T, d, E, R, norm;
+    float *normed, *logits, *eps;  // eps [T][E + 1]: the bounds
     uint32_t* bar;
 };
 
 __global__ __launch_bounds__(FL_T) void k_few_logits(const FewLogitArgs a) {
-    pdl_wait();
     extern __shared__ __align__(16) float s_rows[];
-    __shared__ float s_inv[FEW_T];
-    const int tid = threadIdx.x, d = a.d, pitch = d + 4;
-    const int e0 = blockIdx.x * FL_R, nrow = min(FL_R, a.E + 1 - e0);
-    const int t0 = blockIdx.y * a.group, nt = min(a.group, a.T - t0);
-    float *s_w = s_rows, *s_x = s_rows + FL_R * pitch;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int d = a.d, S = d / 32, pitch = 32 * (S + 4), s4 = S / 4;  // s4 = 8, 16 or 32
+    const int e0 = blockIdx.x * a.R, nrow = min(a.R, a.E + 1 - e0);
+    const int t0 = blockIdx.y * FL_GROUP, nt = min(FL_GROUP, a.T - t0);
+    float *s_x = s_rows, *s_w = s_rows + FL_GROUP * pitch;
+    auto fetch = [&](float* dst, const float* src, int rows) {
+        const int per = d / 4, lg = 31 - __clz(s4);
+        for (int i = tid; i < rows * per; i += FL_T) {
+            const int r = i / per, c = i - r * per;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(
+                             dst + r * pitch + (c >> lg) * (S + 4) + (c & (s4 - 1)) * 4)),
+                         "l"(src + (int64_t)r * d + 4 * c)
+                         : "memory");
+        }
+    };
+    fetch(s_w, a.router + (int64_t)e0 * d, nrow);  // constant weights: before the wait
+    pdl_wait();
+    fetch(s_x, a.x + (int64_t)t0 * d, nt);
     if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) *a.bar = 0;  // of the next kernel
-    for (int i = tid; i < (nrow + nt) * (d / 4); i += FL_T) {
-        const int r = i / (d / 4), c = i - r * (d / 4);
-        const float* src = r < nrow ? a.router + (int64_t)(e0 + r) * d : a.x + (int64_t)(t0 + r - nrow) * d;
-        float* dst = r < nrow ? s_w + r * pitch : s_x + (r - nrow) * pitch;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst + 4 * c)),
-                     "l"(src + 4 * c)
-                     : "memory");
-    }
     asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
     __syncthreads();
     if (a.norm) {
-        // ss = (l0 + l1) + (l2 + l3) over elements 4m + lane, x * (1 / sqrt(ss / d + eps))
-        // (simd.rs:116-137, ops.rs:13-27)
-        if (tid < 4 * FEW_T) {
-            const int t = tid >> 2, l = tid & 3;
-            float acc = 0.0f;
-            if (t < nt) {
-                const float* r = s_x + t * pitch + l;
-#pragma unroll 16
-                for (int j = 0; j < d; j += 4) acc = fadd(acc, fmul(r[j], r[j]));
+        if (warp < nt) {  // x * (1 / sqrt(mean square + eps)), ops.rs:13-27
+            float* r = s_x + warp * pitch + lane * (S + 4);
+            float ss = 0.0f;
+            for (int i = 0; i < S; i += 4) {
+                const float4 v = *reinterpret_cast<const float4*>(r + i);
+                ss = fmaf(v.x, v.x, fmaf(v.y, v.y, fmaf(v.z, v.z, fmaf(v.w, v.w, ss))));
             }
-            const float a1 = __shfl_down_sync(0xffffffffu, acc, 1);
-            const float a2 = __shfl_down_sync(0xffffffffu, acc, 2);
-            const float a3 = __shfl_down_sync(0xffffffffu, acc, 3);
-            if (l == 0) {
-                const float ss = fadd(fadd(acc, a1), fadd(a2, a3));
-                s_inv[t] = fdiv(1.0f, __fsqrt_rn(fadd(fdiv(ss, (float)d), 1e-6f)));
+            const float inv = fdiv(1.0f, __fsqrt_rn(fadd(fdiv(warp_sum(ss), (float)d), 1e-6f)));
+            for (int i = 0; i < S; i += 4) {
+                float4 v = *reinterpret_cast<const float4*>(r + i);
+                v = make_float4(fmul(v.x, inv), fmul(v.y, inv), fmul(v.z, inv), fmul(v.w, inv));
+                *reinterpret_cast<float4*>(r + i) = v;
+                if (blockIdx.x == 0)
+                    *reinterpret_cast<float4*>(a.normed + (int64_t)(t0 + warp) * d + lane * S + i) = v;
             }
         }
         __syncthreads();
-        for (int i = tid; i < nt * (d / 4); i += FL_T) {
-            const int t = i / (d / 4), c = i - t * (d / 4);
-            float4 v = *reinterpret_cast<const float4*>(s_x + t * pitch + 4 * c);
-            const float inv = s_inv[t];
-            v = make_float4(fmul(v.x, inv), fmul(v.y, inv), fmul(v.z, inv), fmul(v.w, inv));
-            *reinterpret_cast<float4*>(s_x + t * pitch + 4 * c) = v;
-            if (blockIdx.x == 0) *reinterpret_cast<float4*>(a.normed + (int64_t)(t0 + t) * d + 4 * c) = v;
+    }
+    for (int q = warp; q < nrow * nt; q += FL_W) {
+        const int r = q / nt, t = q - r * nt, e = e0 + r;
+        const float *wr = s_w + r * pitch + lane * (S + 4), *xr = s_x + t * pitch + lane * (S + 4);
+        float sum = 0.0f, part = 0.0f, terms = 0.0f;
+#pragma unroll 8
+        for (int i = 0; i < S; i += 4) {
+            const float4 w = *reinterpret_cast<const float4*>(wr + i);
+            const float4 v = *reinterpret_cast<const float4*>(xr + i);
+            const float p[4] = {w.x * v.x, w.y * v.y, w.z * v.z, w.w * v.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                sum = fadd(sum, p[j]);
+                part += fabsf(sum);
+                terms += fabsf(p[j]);
+            }
         }
-        __syncthreads();
+        float upto = sum;  // sum of this and the earlier segments
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const float v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        float before = __shfl_up_sync(0xffffffffu, upto, 1);
+        if (lane == 0) before = 0.0f;
+        const float B = warp_sum(fmaf((float)S, fabsf(before), part)), A = warp_sum(terms);
+        const float l = __shfl_sync(0xffffffffu, upto, 31);
+        if (lane == 0) {
+            const float b = a.bias && e < a.E ? a.bias[e] : 0.0f;
+            float bound = 2.2f * B + 12.0f * A + 4.0f * (fabsf(l) + fabsf(b));
+            if (a.norm) bound += ((float)d * 0.125f + 64.0f) * fabsf(l);
+            a.logits[(int64_t)(t0 + t) * (a.E + 1) + e] = l + b;
+            a.eps[(int64_t)(t0 + t) * (a.E + 1) + e] = bound * 5.9604645e-8f;
+        }
     }
-    const int r = tid % FL_R, t = tid / FL_R;
-    if (r >= nrow || t >= nt) return;
-    const float *wr = s_w + r * pitch, *xr = s_x + t * pitch;
-    float acc = 0.0f;
-#pragma unroll 32
-    for (int i = 0; i < d; i += 4) {
-        const float4 w = *reinterpret_cast<const float4*>(wr + i);
-        const float4 v = *reinterpret_cast<const float4*>(xr + i);
-        acc = fadd(acc, fmul(w.x, v.x));
-        acc = fadd(acc, fmul(w.y, v.y));
-        acc = fadd(acc, fmul(w.z, v.z));
-        acc = fadd(acc, fmul(w.w, v.w));
-    }
-    if (a.bias && e0 + r < a.E) acc = fadd(acc, a.bias[e0 + r]);
-    a.logits[(int64_t)(t0 + t) * (a.E + 1) + e0 + r] = acc;
 }
 
 // ---------------------------------------------------------------------------
 // k_few_experts
 // ---------------------------------------------------------------------------
 constexpr int FE_T = 512, FE_W = FE_T / 32;
-constexpr int FE_TB = 4;         // tokens that share a decoded weight
+constexpr int FE_TB = 4;         // tokens at most that share a decoded weight
 constexpr int FE_PART = 512;     // (column group, expert) sums of a CTA kept at a time
-constexpr int FE_MAXU = 513;     // used experts and the shared one
+constexpr int FE_MAXE = 513;     // experts and the shared one (a layer has 512 at most, a thread each)
+constexpr int FE_ITEMS = FE_MAXE + FEW_T / FE_TB;
 
 struct FewExpertArgs {
     const uint8_t *g, *u, *dn, *gs, *us, *dns;       // routed and shared nibbles
     const __half *gd, *ud, *dd, *gsd, *usd, *dsd;    // their block scales
-    const float *x, *xin, *logits;                   // x: the residual; xin: the (normed) input
-    int T, d, f, E, k, has_shared, has_shgate, residual;
+    const float *x, *xin;                            // the residual's and norm's input; the experts'
+    const float *logits, *eps, *router, *bias;
+    int T, d, f, E, k, has_shared, has_shgate, norm, residual;
     int group, n_groups;  // tokens whose inputs a CTA keeps for gate/up; such groups
     float *h, *out;       // h [T][k + shared][f]
     uint32_t *bar, *err;
@@ -266,13 +297,124 @@ PI_DEV bool grid_barrier(uint32_t* bar, uint32_t* err, int* s_ok) {
     return *s_ok != 0;
 }
 
+// Top-k and gates of one token from logits and their bounds, by one warp; false where the
+// bounds leave the reference's choice open. The reference ranks rounded probabilities
+// (model/mod.rs:1278-1303): logits apart by 2^-16 (1 + their distance from the largest) have
+// distinct ones as long as none underflows, hence the second and third conditions. Gates are
+// renormalised over the selected, so the softmax's full sum cancels.
+template <int NPL>
+PI_DEV bool topk_certain(const float* logits, const float* eps, int E, int k, int has_shgate, int32_t* idx,
+                         float* gates, float* share, int lane) {
+    float l[NPL], hi[NPL];
+    uint32_t key[NPL];
+    float m = -INFINITY;
+    bool finite = true;
+#pragma unroll
+    for (int j = 0; j < NPL; ++j) {
+        const int e = lane + 32 * j;
+        l[j] = e < E ? __ldcg(logits + e) : -INFINITY;
+        const float ep = e < E ? __ldcg(eps + e) : 0.0f;
+        hi[j] = l[j] + ep;
+        if (e < E) finite = finite && fabsf(l[j]) < INFINITY && ep < INFINITY;
+        const uint32_t b = __float_as_uint(l[j]);
+        key[j] = e < E ? ((b & 0x80000000u) ? ~b : (b | 0x80000000u)) : 0u;
+        m = fmaxf(m, l[j]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (!__all_sync(0xffffffffu, finite)) return false;
+    int mine = 0x7fffffff;      // lane r: the r-th selected expert, its logit
+    float lm = 0.0f, low = INFINITY;
+    for (int r = 0; r < k; ++r) {
+        uint32_t mk = 0;
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) mk = max(mk, key[j]);
+        mk = __reduce_max_sync(0xffffffffu, mk);
+        uint32_t me = 0xffffffffu;
+#pragma unroll
+        for (int j = NPL - 1; j >= 0; --j)
+            if (key[j] == mk) me = lane + 32 * j;
+        const int e = (int)__reduce_min_sync(0xffffffffu, me);
+        float lo = INFINITY;
+        if ((e & 31) == lane) {
+#pragma unroll
+            for (int j = 0; j < NPL; ++j)
+                if (j == (e >> 5)) {
+                    key[j] = 0;
+                    lo = 2.0f * l[j] - hi[j];
+                    hi[j] = -INFINITY;
+                }
+        }
+        low = fminf(low, __shfl_sync(0xffffffffu, lo, e & 31));
+        if (lane == r) {
+            mine = e;
+            lm = __uint_as_float((mk & 0x80000000u) ? (mk ^ 0x80000000u) : ~mk);
+        }
+    }
+    float high = -INFINITY;  // upper end of those not selected
+#pragma unroll
+    for (int j = 0; j < NPL; ++j) high = fmaxf(high, lane + 32 * j < E ? hi[j] : -INFINITY);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+    if (!(low - m > -80.0f) || !(low > high + 0x1p-16f * (1.0f + (m - low)))) return false;
+    const float p = lane < k ? expf(lm - m) : 0.0f, sum = warp_sum(p);
+    int rank = 0;  // ascending experts, model/mod.rs:1303
+    for (int r = 0; r < k; ++r) rank += __shfl_sync(0xffffffffu, mine, r) < mine;
+    if (lane < k) {
+        idx[rank] = mine;
+        gates[rank] = p / sum;
+    }
+    if (lane == 0) *share = has_shgate ? 1.0f / (1.0f + expf(-__ldcg(logits + E))) : 1.0f;
+    return true;
+}
+
+// The reference's logits of one token, by the whole CTA: its norm (four sequential sums of
+// squares, simd.rs:116-137) and one sequential chain a thread. Only for tokens that
+// topk_certain leaves open.
+PI_DEV void exact_logits(const float* x, const float* router, const float* bias, int d, int E, int norm,
+                         float* out, float* s_inv) {
+    const int tid = threadIdx.x;
+    if (norm && tid < 32) {
+        float acc = 0.0f;
+        if (tid < 4)
+#pragma unroll 16
+            for (int j = tid; j < d; j += 4) acc = fadd(acc, fmul(x[j], x[j]));
+        const float a1 = __shfl_sync(0xffffffffu, acc, 1), a2 = __shfl_sync(0xffffffffu, acc, 2),
+                    a3 = __shfl_sync(0xffffffffu, acc, 3);
+        if (tid == 0) {
+            const float ss = fadd(fadd(acc, a1), fadd(a2, a3));
+            *s_inv = fdiv(1.0f, __fsqrt_rn(fadd(fdiv(ss, (float)d), 1e-6f)));
+        }
+    }
+    __syncthreads();
+    const float inv = norm ? *s_inv : 1.0f;
+    for (int e = tid; e <= E; e += FE_T) {
+        const float* w = router + (int64_t)e * d;
+        float acc = 0.0f;
+#pragma unroll 8
+        for (int i = 0; i < d; i += 4) {
+            const float4 a = __ldg(reinterpret_cast<const float4*>(w + i));
+            float4 v = *reinterpret_cast<const float4*>(x + i);
+            if (norm) v = make_float4(fmul(v.x, inv), fmul(v.y, inv), fmul(v.z, inv), fmul(v.w, inv));
+            acc = fadd(acc, fmul(a.x, v.x));
+            acc = fadd(acc, fmul(a.y, v.y));
+            acc = fadd(acc, fmul(a.z, v.z));
+            acc = fadd(acc, fmul(a.w, v.w));
+        }
+        out[e] = bias && e < E ? fadd(acc, bias[e]) : acc;
+    }
+    __syncthreads();
+}
+
 template <int CPL, int NPL>
 __global__ __launch_bounds__(FE_T, 1) void k_few_experts(const FewExpertArgs a) {
-    extern __shared__ __align__(16) float s_dyn[];  // gate/up: inputs of the group's tokens, then top-k scratch; down: h
-    __shared__ int s_idx[FEW_T * 32], s_sel[FE_W][32], s_use[FE_MAXU], s_mask[FE_MAXU], s_nuse, s_ok;
-    __shared__ float s_gate[FEW_T * 32], s_share[FEW_T], s_part[FE_PART * 8];
+    extern __shared__ __align__(16) float s_dyn[];  // gate/up: inputs of the group's tokens; down: h
+    __shared__ int s_idx[FEW_T * 32], s_use[FE_ITEMS], s_mask[FE_T], s_item[FE_ITEMS], s_count[FE_W], s_nuse, s_ok;
+    __shared__ uint32_t s_open;
+    __shared__ float s_gate[FEW_T * 32], s_share[FEW_T], s_inv, s_part[FE_PART * 8];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int T = a.T, d = a.d, f = a.f, E = a.E, k = a.k, nb = d / 32, slots = k + a.has_shared;
+    constexpr int d = 1024 * CPL, nb = d / 32;
+    const int T = a.T, f = a.f, E = a.E, k = a.k, slots = k + a.has_shared;
     const int grp = blockIdx.x % a.n_groups, t0 = grp * a.group, nt = min(a.group, T - t0);
     const int cta = blockIdx.x / a.n_groups, n_cta = (gridDim.x - grp + a.n_groups - 1) / a.n_groups;
 
@@ -286,86 +428,145 @@ __global__ __launch_bounds__(FE_T, 1) void k_few_experts(const FewExpertArgs a) 
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
     // routing of every token (a warp each), in every CTA
-    if (warp < T)
-        topk_token<NPL>(a.logits, warp, E, k, a.has_shgate, s_idx, s_gate, s_share, nullptr,
-                        s_dyn + a.group * nb * 36 + warp * 32 * NPL, s_sel[warp], lane);
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    // the experts that the group's tokens use, ascending, with the tokens of each
-    for (int e = tid; e < E; e += FE_T) s_mask[e] = 0;
+    if (tid == 0) s_open = 0;
+    s_mask[tid] = 0;
     __syncthreads();
+    if (warp < T &&
+        !topk_certain<NPL>(a.logits + (int64_t)warp * (E + 1), a.eps + (int64_t)warp * (E + 1), E, k, a.has_shgate,
+                           s_idx + warp * k, s_gate + warp * k, s_share + warp, lane) &&
+        lane == 0)
+        atomicOr(&s_open, 1u << warp);
+    __syncthreads();
+    for (uint32_t open = s_open; open; open &= open - 1) {
+        // s_part: the token's logits, then the scratch of its top-k
+        const int t = __ffs(open) - 1;
+        exact_logits(a.x + (int64_t)t * d, a.router, a.bias, d, E, a.norm, s_part, &s_inv);
+        if (warp == 0)
+            topk_token<NPL, true>(s_part, 0, E, k, a.has_shgate, s_idx + t * k, s_gate + t * k, s_share + t, nullptr,
+                                  s_part + FE_MAXE, s_item, lane);
+        __syncthreads();
+    }
+    // What this CTA's part of the down projection will read goes to L2 meanwhile (T = 1: the
+    // phase behind the barrier took 4.7 us, most of it the first trip to memory).
+    const int per_tok = d / 8, bpq = f / 128, hp = f + 16;  // hp: floats of a padded h row
+    const int64_t all = (int64_t)T * per_tok;
+    const int ub = (int)(all * blockIdx.x / gridDim.x), ue = (int)(all * (blockIdx.x + 1) / gridDim.x);
+    {
+        const int lines = f / 32 + max(1, f / 256);  // 128-byte lines of eight rows: 4 f of nibbles, f / 2 of scales
+        const int v0 = ub + warp / 2;                // 16 lanes take the pieces of a unit
+        for (int v = v0; v < ue; v += FE_W / 2) {
+            const int t = v / per_tok, c0 = (v - t * per_tok) * 8;
+            for (int j = 0; j < slots; ++j) {
+                const int e = j < k ? s_idx[t * k + j] : E;
+                const int64_t row = (e == E ? 0 : (int64_t)e * d) + c0;
+                const uint8_t* D = (e == E ? a.dns : a.dn) + row * (f / 2);
+                const uint8_t* DD = reinterpret_cast<const uint8_t*>((e == E ? a.dsd : a.dd) + row * (f / 32));
+                const int l = (warp & 1) * 32 + lane;
+                if (l < lines)
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(l < f / 32 ? D + l * 128 : DD + (l - f / 32) * 128));
+            }
+        }
+    }
+    // The group's work: items of an expert and up to four of its tokens, which share the decoded
+    // weights. The shared expert's come first, then those of several tokens, so that the
+    // heaviest are spread evenly over the warps. Thread e counts the items of expert e.
     for (int i = tid; i < nt * k; i += FE_T) atomicOr(&s_mask[s_idx[t0 * k + i]], 1 << (i / k));
     __syncthreads();
-    if (warp == 0) {
-        int n = 0;
-        for (int e0 = 0; e0 < E; e0 += 32) {
-            const int m = e0 + lane < E ? s_mask[e0 + lane] : 0;
-            const uint32_t b = __ballot_sync(0xffffffffu, m != 0);
-            if (m) s_use[n + __popc(b & ((1u << lane) - 1u))] = e0 + lane;
-            n += __popc(b);
+    {
+        const int n_sh = a.has_shared ? (nt + FE_TB - 1) / FE_TB : 0;
+        int m = tid < E ? s_mask[tid] : 0;
+        const int p = __popc(m), mine = p == 1 ? 1 << 16 : (p + FE_TB - 1) / FE_TB;  // light << 16 | heavy
+        int upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
         }
-        if (a.has_shared && lane == 0) {
-            s_use[n] = E;
-            s_mask[E] = (1 << nt) - 1;
+        if (lane == 31) s_count[warp] = upto;
+        __syncthreads();
+        int before = 0, total = 0;
+#pragma unroll
+        for (int w = 0; w < FE_W; ++w) {
+            const int c = s_count[w];
+            if (w < warp) before += c;
+            total += c;
         }
-        if (lane == 0) s_nuse = n + a.has_shared;
+        before += upto - mine;
+        const int heavy = total & 0xffff;
+        int at = n_sh + (p == 1 ? heavy + (before >> 16) : (before & 0xffff));
+        for (; m; ++at) {
+            int take = 0;
+            for (int i = 0; i < FE_TB && m; ++i) {
+                take |= m & -m;
+                m &= m - 1;
+            }
+            s_use[at] = tid;
+            s_item[at] = take;
+        }
+        if (tid < n_sh) {
+            s_use[tid] = E;
+            s_item[tid] = ((1 << min(FE_TB, nt - FE_TB * tid)) - 1) << (FE_TB * tid);
+        }
+        if (tid == 0) s_nuse = n_sh + heavy + (total >> 16);
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
 
-    // gate, up and SwiGLU: a warp takes two rows of an expert for all of its tokens
+    // gate, up and SwiGLU: a warp takes two rows of an expert for the tokens of an item
     const int half_f = f / 2, n_unit = s_nuse * half_f;
     for (int unit = cta * FE_W + warp; unit < n_unit; unit += n_cta * FE_W) {
-        const int e = s_use[unit / half_f], row = 2 * (unit % half_f);
+        const int item = unit / half_f, e = s_use[item], row = 2 * (unit - item * half_f);
         const bool sh = e == E;
-        uint32_t mask = s_mask[e];
+        uint32_t mask = s_item[item];
         const int64_t r = (sh ? 0 : (int64_t)e * f) + row;
         const uint8_t *G = (sh ? a.gs : a.g) + r * (d / 2), *U = (sh ? a.us : a.u) + r * (d / 2);
         const __half *GD = (sh ? a.gsd : a.gd) + r * nb, *UD = (sh ? a.usd : a.ud) + r * nb;
-        auto store = [&](int t, const float (&g)[2], const float (&u)[2]) {  // lanes 0, 1: a row each
-            int j = k;
-            if (!sh) j = __ffs(__ballot_sync(0xffffffffu, lane < k && s_idx[(t0 + t) * k + lane] == e)) - 1;
-            if (lane < 2)
-                a.h[((int64_t)(t0 + t) * slots + j) * f + row + lane] =
-                    swiglu_ref(lane ? g[1] : g[0], lane ? u[1] : u[0]);
-        };
-        if (__popc(mask) == 1) {
-            const int t = __ffs(mask) - 1;
-            const float* xs[1] = {s_dyn + t * nb * 36};
-            float sum[4][1];
-            gateup_rows<CPL, 1>(G, U, GD, UD, d, xs, lane, sum);
-            const float g[2] = {sum[0][0], sum[2][0]}, u[2] = {sum[1][0], sum[3][0]};
-            store(t, g, u);
-        } else {
-            while (mask) {
-                int tok[FE_TB], n = 0;
-                const float* xs[FE_TB];
+        int tok[FE_TB], n = 0;
+        const float* xs[FE_TB];
 #pragma unroll
-                for (int i = 0; i < FE_TB; ++i) {  // a batch that is not full repeats its last token
-                    if (mask) {
-                        tok[i] = __ffs(mask) - 1;
-                        mask &= mask - 1;
-                        ++n;
-                    } else {
-                        tok[i] = tok[i > 0 ? i - 1 : 0];
-                    }
-                    xs[i] = s_dyn + tok[i] * nb * 36;
-                }
-                float sum[4][FE_TB];
-                gateup_rows<CPL, FE_TB>(G, U, GD, UD, d, xs, lane, sum);
-#pragma unroll
-                for (int i = 0; i < FE_TB; ++i) {
-                    if (i >= n) break;
-                    const float g[2] = {sum[0][i], sum[2][i]}, u[2] = {sum[1][i], sum[3][i]};
-                    store(tok[i], g, u);
-                }
+        for (int i = 0; i < FE_TB; ++i) {  // an item that is not full repeats its last token
+            if (mask) {
+                tok[i] = __ffs(mask) - 1;
+                mask &= mask - 1;
+                ++n;
+            } else {
+                tok[i] = tok[i > 0 ? i - 1 : 0];
             }
+            xs[i] = s_dyn + tok[i] * nb * 36;
+        }
+        float sum[4][FE_TB];
+        if (n == 1) {
+            float s1[4][1];
+            const float* const x1[1] = {xs[0]};
+            gateup_rows<CPL, 1>(G, U, GD, UD, d, x1, lane, s1);
+#pragma unroll
+            for (int v = 0; v < 4; ++v) sum[v][0] = s1[v][0];
+        } else if (n == 2) {
+            float s2[4][2];
+            const float* const x2[2] = {xs[0], xs[1]};
+            gateup_rows<CPL, 2>(G, U, GD, UD, d, x2, lane, s2);
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                sum[v][0] = s2[v][0];
+                sum[v][1] = s2[v][1];
+            }
+        } else {
+            gateup_rows<CPL, FE_TB>(G, U, GD, UD, d, xs, lane, sum);
+        }
+#pragma unroll
+        for (int i = 0; i < FE_TB; ++i) {
+            if (i >= n) break;
+            const int t = t0 + tok[i];
+            int j = k;
+            if (!sh) j = __ffs(__ballot_sync(0xffffffffu, lane < k && s_idx[t * k + lane] == e)) - 1;
+            if (lane < 2)
+                a.h[((int64_t)t * slots + j) * f + row + lane] =
+                    swiglu_ref(lane ? sum[2][i] : sum[0][i], lane ? sum[3][i] : sum[1][i]);
         }
     }
     if (!grid_barrier(a.bar, a.err, &s_ok)) return;
 
     // down: the CTA's share of the (token, eight columns) units, token by token
-    const int per_tok = d / 8, bpq = f / 128, hp = f + 16;  // hp: floats of a padded h row
-    const int64_t all = (int64_t)T * per_tok;
-    const int ub = (int)(all * blockIdx.x / gridDim.x), ue = (int)(all * (blockIdx.x + 1) / gridDim.x);
     for (int u = ub; u < ue;) {
         const int t = u / per_tok, tok_end = min(ue, (t + 1) * per_tok);
         __syncthreads();
@@ -411,10 +612,10 @@ __global__ __launch_bounds__(FE_T, 1) void k_few_experts(const FewExpertArgs a) 
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
-constexpr size_t FEW_X_BYTES = 152 * 1024;  // inputs of the tokens a CTA keeps for gate/up
+constexpr size_t FEW_X_BYTES = 180 * 1024;  // inputs of the tokens a CTA keeps for gate/up
 
 struct FewBufs {
-    float *logits, *normed, *h;
+    float *logits, *eps, *normed, *h;
     uint32_t* bar;
     size_t bytes;
 };
@@ -423,6 +624,7 @@ FewBufs few_carve(const pi_moe_layer* L, int64_t T, char* base) {
     FewBufs o;
     o.bar = b.take<uint32_t>(1);
     o.logits = b.take<float>(T * (L->E + 1));
+    o.eps = b.take<float>(T * (L->E + 1));
     o.normed = b.take<float>(T * L->d);
     o.h = b.take<float>(T * (L->k + (L->has_shared ? 1 : 0)) * L->f);
     o.bytes = b.off + 256;
@@ -431,8 +633,8 @@ FewBufs few_carve(const pi_moe_layer* L, int64_t T, char* base) {
 
 template <int CPL, int NPL>
 cudaError_t launch_experts(const FewExpertArgs& a, int sms, cudaStream_t st) {
-    const size_t x = (size_t)a.group * (a.d / 32) * 36 * 4, p = (size_t)FE_W * 32 * NPL * 4;
-    const size_t h = (size_t)(a.k + a.has_shared) * (a.f + 16) * 4, smem = std::max(x + p, h);
+    const size_t x = (size_t)a.group * (a.d / 32) * 36 * 4;
+    const size_t h = (size_t)(a.k + a.has_shared) * (a.f + 16) * 4, smem = std::max(x, h);
     auto kern = k_few_experts<CPL, NPL>;
     // the limit is always raised: beside the kernel's 26 KB of static shared memory the default
     // of 48 KB would not hold what pi_smem_attr lets pass as small
@@ -473,13 +675,15 @@ int few_forward(pi_ctx* ctx, const pi_moe_layer* L, const float* x, int64_t T, f
     const bool norm = flags & PI_FWD_RMSNORM;
     {
         PiProfScope ps(ctx, st, "k_few_logits");
-        // tokens of a CTA: what 128 KB of shared memory hold
-        const int group = (int)std::min<int64_t>(T, (128 * 1024) / (4 * d));
-        const size_t smem = sizeof(float) * (size_t)(FL_R + group) * (d + 4);
+        // rows of a CTA: two at least, more where that still gives every SM a CTA and the rows fit
+        const int64_t sms = ctx->sm_count > 0 ? ctx->sm_count : 148, groups = (T + FL_GROUP - 1) / FL_GROUP;
+        const size_t row = sizeof(float) * (size_t)(d + 128);
+        const int fit = (int)(FL_SMEM / row) - FL_GROUP;
+        const int R = (int)std::min<int64_t>(fit, std::max<int64_t>(2, ((E + 1) * groups + sms - 1) / sms));
+        const size_t smem = row * (FL_GROUP + R);
         pi_smem_attr((const void*)k_few_logits, smem);
-        const FewLogitArgs a{x, L->router, L->bias, (int)T, d, E, group, norm ? 1 : 0, B.normed, B.logits, B.bar};
-        pi_pdl_launch(k_few_logits, dim3((unsigned)((E + FL_R) / FL_R), (unsigned)((T + group - 1) / group)),
-                      dim3(FL_T), smem, st, a);
+        const FewLogitArgs a{x, L->router, L->bias, (int)T, d, E, R, norm ? 1 : 0, B.normed, B.logits, B.eps, B.bar};
+        pi_pdl_launch(k_few_logits, dim3((unsigned)((E + R) / R), (unsigned)groups), dim3(FL_T), smem, st, a);
         if (int rc = pi_cuda_check(ctx, cudaGetLastError(), "moe fused logits")) return rc;
     }
     PiProfScope ps(ctx, st, "k_few_experts");
@@ -502,6 +706,10 @@ int few_forward(pi_ctx* ctx, const pi_moe_layer* L, const float* x, int64_t T, f
     a.x = x;
     a.xin = norm ? B.normed : x;
     a.logits = B.logits;
+    a.eps = B.eps;
+    a.router = L->router;
+    a.bias = L->bias;
+    a.norm = norm ? 1 : 0;
     a.T = (int)T;
     a.d = d;
     a.f = (int)L->f;
