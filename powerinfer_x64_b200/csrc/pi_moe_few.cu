@@ -13,13 +13,15 @@
 // tokens for normal inputs, and exact ties) is made again from sequential logits and the
 // reference's own softmax and top-k (pi_topk.cuh).
 //
-// Expert products are f32 sums of f32 activations and the exact nibble values, one multiply
-// by the block's scale per 32 terms (the reference dequantises and sums sequentially,
-// quant/mod.rs:958-969): equal to f32 rounding, as on the layer's other Q4_0 paths.
+// Expert products: the reference dequantises Q4_0 rows and sums f32 products (quant/mod.rs:
+// 958-969). Here 32 inputs that share a weight scale become fixed-point numbers of 22 bits
+// below their largest, held as three int8 terms, so a block's dot with the nibbles is three
+// exact integer dots (dp4a: 1.1 instructions a weight and token, against 2.4 for decoding
+// nibbles to f32), and one f32 multiply-add per block follows. An input is then within 2^-22 of
+// its block's largest, which moves a sum by no more than f32 products and sums do.
 //
 // Bound: the bytes of the experts that the tokens use; for a token or two the latency of the
-// chain (two launches, the barrier and four dependent trips to memory), for many tokens the
-// decoding of nibbles on the integer pipe. k_few_experts is launched cooperatively: its
+// chain (two launches, the barrier and four dependent trips to memory). k_few_experts is launched cooperatively: its
 // barrier needs every CTA resident, also while another stream runs the same.
 #include "pi_common.cuh"
 #include "pi_internal.h"
@@ -31,6 +33,50 @@
 namespace {
 
 constexpr int FEW_T = 16;  // tokens at most
+
+// ---------------------------------------------------------------------------
+// Fixed-point blocks. 32 values in eight lanes, four each: with 2^e the power of two that
+// brings the largest into [2^21, 2^22), X = rint(x 2^e) = 65536 q1 + 256 q2 + q3, each q an
+// int8. A block is 28 words: [term][word of eight elements][even elements, odd elements], as
+// the nibbles of a Q4_0 word fall apart (low: even, high: odd), then the scale 2^-e / 16
+// (nibbles come shifted by four bits), then padding that keeps the lanes' 16-byte reads of
+// neighbouring blocks in distinct banks. A NaN or infinity makes the block's scale NaN.
+// ---------------------------------------------------------------------------
+constexpr int FX_WORDS = 28;
+
+// v: this lane's elements 4j..4j+3 of a block, j = lane % 8; all 32 lanes call it
+PI_DEV void fix_block(const float4 v, uint32_t* blk, int j, bool store) {
+    float m = max_nan(max_nan(fabsf(v.x), fabsf(v.y)), max_nan(fabsf(v.z), fabsf(v.w)));
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const bool fin = m < INFINITY;
+    const int ex = fin && m > 0.0f ? min(21 - ilogbf(m), 120) : 0;
+    const float s = fin ? ldexpf(1.0f, ex) : 0.0f, e[4] = {v.x, v.y, v.z, v.w};
+    uint32_t even[3] = {0, 0, 0}, odd[3] = {0, 0, 0};  // two bytes of each term
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int X = fin ? __float2int_rn(e[i] * s) : 0;
+        const int q3 = (int)(int8_t)X, X2 = (X - q3) >> 8, q2 = (int)(int8_t)X2, q1 = (X2 - q2) >> 8;
+        uint32_t* to = i & 1 ? odd : even;
+        to[0] |= (uint32_t)(q1 & 255) << (8 * (i >> 1));
+        to[1] |= (uint32_t)(q2 & 255) << (8 * (i >> 1));
+        to[2] |= (uint32_t)(q3 & 255) << (8 * (i >> 1));
+    }
+    if (!store) return;
+    uint16_t* h = reinterpret_cast<uint16_t*>(blk);
+#pragma unroll
+    for (int t = 0; t < 3; ++t) {
+        h[t * 16 + (j >> 1) * 4 + (j & 1)] = (uint16_t)even[t];
+        h[t * 16 + (j >> 1) * 4 + 2 + (j & 1)] = (uint16_t)odd[t];
+    }
+    if (j == 0) blk[24] = __float_as_uint(fin ? ldexpf(0.0625f, -ex) : __int_as_float(0x7fffffff));
+}
+
+// nibbles of a word as 16 (n - 8) in int8: even elements, odd elements
+PI_DEV uint32_t nib_even(uint32_t w) { return ((w << 4) & 0xF0F0F0F0u) ^ 0x80808080u; }
+PI_DEV uint32_t nib_odd(uint32_t w) { return (w & 0xF0F0F0F0u) ^ 0x80808080u; }
+// the value of a block's three dots
+PI_DEV float fix_value(const int (&s)[3]) { return fmaf((float)s[0], 65536.0f, (float)(s[1] * 256 + s[2])); }
 
 // ---------------------------------------------------------------------------
 // k_few_logits: CTA = R router rows (row E: the shared expert's gate) and a group of tokens in
@@ -54,8 +100,8 @@ constexpr size_t FL_SMEM = 190 * 1024;
 struct FewLogitArgs {
     const float *x, *router, *bias;
     int T, d, E, R, norm;
-    float *normed, *logits, *eps;  // eps [T][E + 1]: the bounds
-    uint32_t* bar;
+    float *logits, *eps;  // [T][E + 1], eps: the bounds
+    uint32_t *xfix, *bar;  // xfix [T][d / 32][FX_WORDS]: the (normed) inputs in fixed point
 };
 
 __global__ __launch_bounds__(FL_T) void k_few_logits(const FewLogitArgs a) {
@@ -94,11 +140,17 @@ __global__ __launch_bounds__(FL_T) void k_few_logits(const FewLogitArgs a) {
                 float4 v = *reinterpret_cast<const float4*>(r + i);
                 v = make_float4(fmul(v.x, inv), fmul(v.y, inv), fmul(v.z, inv), fmul(v.w, inv));
                 *reinterpret_cast<float4*>(r + i) = v;
-                if (blockIdx.x == 0)
-                    *reinterpret_cast<float4*>(a.normed + (int64_t)(t0 + warp) * d + lane * S + i) = v;
             }
         }
         __syncthreads();
+    }
+    // the blocks of the group's inputs are shared out over the CTAs of the group
+    for (int q0 = 0; q0 * (int)gridDim.x < nt * (d / 32); q0 += FL_T / 8) {
+        const int o = (q0 + (tid >> 3)) * gridDim.x + blockIdx.x, j = tid & 7;
+        const bool in = o < nt * (d / 32);
+        const int t = in ? o / (d / 32) : 0, b = in ? o - t * (d / 32) : 0, i = b * 32 + 4 * j;
+        const float4 v = *reinterpret_cast<const float4*>(s_x + t * pitch + (i / S) * (S + 4) + (i & (S - 1)));
+        fix_block(v, a.xfix + ((int64_t)(t0 + t) * (d / 32) + b) * FX_WORDS, j, in);
     }
     for (int q = warp; q < nrow * nt; q += FL_W) {
         const int r = q / nt, t = q - r * nt, e = e0 + r;
@@ -148,7 +200,8 @@ constexpr int FE_ITEMS = FE_MAXE + FEW_T / FE_TB;
 struct FewExpertArgs {
     const uint8_t *g, *u, *dn, *gs, *us, *dns;       // routed and shared nibbles
     const __half *gd, *ud, *dd, *gsd, *usd, *dsd;    // their block scales
-    const float *x, *xin;                            // the residual's and norm's input; the experts'
+    const float* x;                                  // the layer's input
+    const uint32_t* xfix;
     const float *logits, *eps, *router, *bias;
     int T, d, f, E, k, has_shared, has_shgate, norm, residual;
     int group, n_groups;  // tokens whose inputs a CTA keeps for gate/up; such groups
@@ -156,121 +209,155 @@ struct FewExpertArgs {
     uint32_t *bar, *err;
 };
 
-// Eight nibbles of a word (element 2i low, 2i + 1 high in byte i) as pairs of f32: a byte
-// put below 0x4B000000 is the float 2^23 + n, from which 2^23 + 8 is taken exactly.
-PI_DEV void nibble_pairs(uint32_t w, uint64_t* v) {
-    const uint32_t lo = w & 0x0F0F0F0Fu, hi = (w >> 4) & 0x0F0F0F0Fu;
-    const uint64_t off = pack2(-8388616.0f, -8388616.0f);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        v[i] = add2(pack2(__uint_as_float(__byte_perm(lo, 0x4B000000u, 0x7440 + i)),
-                          __uint_as_float(__byte_perm(hi, 0x4B000000u, 0x7440 + i))),
-                    off);
-}
 PI_DEV uint32_t word_of(const int4& v, int i) {
     return (uint32_t)(i == 0 ? v.x : (i == 1 ? v.y : (i == 2 ? v.z : v.w)));
 }
 
-// Gate and up of two neighbouring rows for TB tokens: lane l holds blocks l + 32 c of each row.
-// xs[t]: the token's inputs in shared memory, 36 floats a block (lanes' 16-byte reads then
-// fall into distinct banks). sum[2 row + (0 gate, 1 up)][token], over all lanes.
-template <int CPL, int TB>
-PI_DEV void gateup_rows(const uint8_t* G, const uint8_t* U, const __half* GD, const __half* UD, int d,
-                        const float* const (&xs)[TB], int lane, float (&sum)[4][TB]) {
-    int4 w[2][4];
-    float s[2][4];
-    const int nb = d / 32;
-    auto load = [&](int c, int4 (&q)[4], float (&sc)[4]) {
+// Gate and up of two neighbouring rows: where they start, and one chunk (the lane's block
+// l + 32 c of each row) in registers.
+struct RowPtrs {
+    const uint8_t *g, *u;
+    const __half *gd, *ud;
+};
+struct RowChunk {
+    int4 w[4];  // row 0 gate, up, row 1 gate, up
+    __half s[4];
+    PI_DEV void load(const RowPtrs& p, int nb, int blk) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            const int64_t b = (int64_t)r * nb + lane + 32 * c;
-            q[2 * r] = ld_stream(G + b * 16);
-            q[2 * r + 1] = ld_stream(U + b * 16);
-            sc[2 * r] = __half2float(GD[b]);
-            sc[2 * r + 1] = __half2float(UD[b]);
+            const int b = r * nb + blk;
+            w[2 * r] = ld_stream(p.g + b * 16);
+            w[2 * r + 1] = ld_stream(p.u + b * 16);
+            s[2 * r] = p.gd[b];
+            s[2 * r + 1] = p.ud[b];
         }
-    };
+    }
+};
+
+// sum[v][t] += row-vector v of the chunk times token t's block (xs[t]: the token's fixed-point
+// blocks in shared memory).
+template <int TB>
+PI_DEV void chunk_products(const RowChunk& k, const uint32_t* const (&xs)[TB], int blk, float (&sum)[4][TB]) {
+    int dot[4][TB][3];
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+#pragma unroll
+        for (int t = 0; t < TB; ++t) dot[v][t][0] = dot[v][t][1] = dot[v][t][2] = 0;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {  // two words, sixteen elements
+        uint32_t n[4][4];
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t x = word_of(k.w[v], 2 * q + i);
+                n[v][2 * i] = nib_even(x);
+                n[v][2 * i + 1] = nib_odd(x);
+            }
+#pragma unroll
+        for (int t = 0; t < TB; ++t)
+#pragma unroll
+            for (int p = 0; p < 3; ++p) {
+                const int4 x = *reinterpret_cast<const int4*>(xs[t] + blk * FX_WORDS + p * 8 + q * 4);
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    int& o = dot[v][t][p];
+                    o = dp4a((int)n[v][0], x.x, o);
+                    o = dp4a((int)n[v][1], x.y, o);
+                    o = dp4a((int)n[v][2], x.z, o);
+                    o = dp4a((int)n[v][3], x.w, o);
+                }
+            }
+    }
+#pragma unroll
+    for (int t = 0; t < TB; ++t) {
+        const float sx = __uint_as_float(xs[t][blk * FX_WORDS + 24]);
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+            sum[v][t] = fmaf(__half2float(k.s[v]) * sx, fix_value(dot[v][t]), sum[v][t]);
+    }
+}
+
+// All chunks of a unit for TB tokens, the unit's first chunk being in `k`; leaves there the first
+// chunk of the next unit (at `next`), which is on its way while the last one is worked on.
+// sum[t]: lanes 0-7 the first row's gate, 8-15 its up, 16-23 the second row's gate, 24-31 its up.
+template <int CPL, int TB>
+PI_DEV void gateup_rows(RowChunk& k, const RowPtrs& at, const RowPtrs& next, const uint32_t* const (&xs)[TB],
+                        int lane, float* out) {
+    constexpr int nb = 32 * CPL;
+    RowChunk other;
+    float sum[4][TB];
 #pragma unroll
     for (int v = 0; v < 4; ++v)
 #pragma unroll
         for (int t = 0; t < TB; ++t) sum[v][t] = 0.0f;
-    load(0, w[0], s[0]);
 #pragma unroll
     for (int c = 0; c < CPL; ++c) {
-        if (c + 1 < CPL) load(c + 1, w[(c + 1) & 1], s[(c + 1) & 1]);
-        uint64_t part[4][TB];
-#pragma unroll
-        for (int v = 0; v < 4; ++v)
-#pragma unroll
-            for (int t = 0; t < TB; ++t) part[v][t] = 0;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {  // words: eight elements
-            uint64_t n[4][4];
-#pragma unroll
-            for (int v = 0; v < 4; ++v) nibble_pairs(word_of(w[c & 1][v], q), n[v]);
-#pragma unroll
-            for (int t = 0; t < TB; ++t) {
-                const ulonglong2* xp = reinterpret_cast<const ulonglong2*>(xs[t] + (lane + 32 * c) * 36 + q * 8);
-                const ulonglong2 x0 = xp[0], x1 = xp[1];
-#pragma unroll
-                for (int v = 0; v < 4; ++v) {
-                    part[v][t] = fma2(n[v][0], x0.x, part[v][t]);
-                    part[v][t] = fma2(n[v][1], x0.y, part[v][t]);
-                    part[v][t] = fma2(n[v][2], x1.x, part[v][t]);
-                    part[v][t] = fma2(n[v][3], x1.y, part[v][t]);
-                }
-            }
-        }
-#pragma unroll
-        for (int v = 0; v < 4; ++v)
-#pragma unroll
-            for (int t = 0; t < TB; ++t) {
-                const float2 p = unpack2(part[v][t]);
-                sum[v][t] = fmaf(s[c & 1][v], p.x + p.y, sum[v][t]);
-            }
+        RowChunk &now = c & 1 ? other : k, &then = c & 1 ? k : other;
+        if (c + 1 < CPL) then.load(at, nb, lane + 32 * (c + 1));
+        else then.load(next, nb, lane);
+        chunk_products<TB>(now, xs, lane + 32 * c, sum);
     }
+    if (CPL & 1) k = other;
+    // sums over the lanes, four at once: after two halvings lane l has row-vector l / 8's part
 #pragma unroll
-    for (int v = 0; v < 4; ++v)
+    for (int t = 0; t < TB; ++t) {
+        const bool hi = lane & 16, mid = lane & 8;
+        float a = hi ? sum[2][t] : sum[0][t], b = hi ? sum[3][t] : sum[1][t];
+        a += __shfl_xor_sync(0xffffffffu, hi ? sum[0][t] : sum[2][t], 16);
+        b += __shfl_xor_sync(0xffffffffu, hi ? sum[1][t] : sum[3][t], 16);
+        float c = mid ? b : a;
+        c += __shfl_xor_sync(0xffffffffu, mid ? a : b, 8);
 #pragma unroll
-        for (int t = 0; t < TB; ++t) sum[v][t] = warp_sum(sum[v][t]);
+        for (int o = 4; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
+        out[t] = c;
+    }
 }
 
-// One expert's part of eight output columns (rows of D, lane-tiled by quarters of a row):
-// lane 4 r + q sums quarter q of row r; returns the row's sum in its lanes. hq: h in shared
-// memory, quarter q at q (8 BPQ * 4 + 4) floats.
+// h of one expert in shared memory: BPQ fixed-point blocks per quarter of a row, the quarters
+// apart so that the four lanes of a row read distinct banks.
+PI_DEV int h_quarter(int bpq) { return bpq * FX_WORDS + (bpq == 1 ? 0 : 4); }
+
+// One expert's part of eight output columns (rows of D, lane-tiled by quarters of a row): the
+// lane's blocks in registers, and their sum. Lane 4 r + q sums quarter q of row r; the row's
+// sum is returned in its lanes.
 template <int BPQ>
-PI_DEV float down_rows(const uint8_t* D, const __half* DD, const float* hs, int lane) {
-    const int r = lane >> 2, q = lane & 3;
+struct DownRows {
     int4 w[BPQ];
-    float s[BPQ];
+    __half s[BPQ];
+    PI_DEV void load(const uint8_t* D, const __half* DD, int lane) {
 #pragma unroll
-    for (int b = 0; b < BPQ; ++b) {
-        w[b] = ld_stream(D + (b * 32 + lane) * 16);
-        s[b] = __half2float(DD[(r * 4 + q) * BPQ + b]);
-    }
-    const float* hp = hs + q * (BPQ * 32 + 4);
-    float sum = 0.0f;
-#pragma unroll
-    for (int b = 0; b < BPQ; ++b) {
-        uint64_t part = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint64_t n[4];
-            nibble_pairs(word_of(w[b], i), n);
-            const ulonglong2* x = reinterpret_cast<const ulonglong2*>(hp + b * 32 + i * 8);
-            const ulonglong2 x0 = x[0], x1 = x[1];
-            part = fma2(n[0], x0.x, part);
-            part = fma2(n[1], x0.y, part);
-            part = fma2(n[2], x1.x, part);
-            part = fma2(n[3], x1.y, part);
+        for (int b = 0; b < BPQ; ++b) {
+            w[b] = ld_stream(D + (b * 32 + lane) * 16);
+            s[b] = DD[lane * BPQ + b];
         }
-        const float2 p = unpack2(part);
-        sum = fmaf(s[b], p.x + p.y, sum);
     }
-    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-    return sum;
-}
+    PI_DEV float sum(const uint32_t* hs, int lane) const {
+        const uint32_t* hp = hs + (lane & 3) * h_quarter(BPQ);
+        float sum = 0.0f;
+#pragma unroll
+        for (int b = 0; b < BPQ; ++b) {
+            int dot[3] = {0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t w0 = word_of(w[b], 2 * i), w1 = word_of(w[b], 2 * i + 1);
+                const uint32_t n[4] = {nib_even(w0), nib_odd(w0), nib_even(w1), nib_odd(w1)};
+#pragma unroll
+                for (int p = 0; p < 3; ++p) {
+                    const int4 x = *reinterpret_cast<const int4*>(hp + b * FX_WORDS + p * 8 + i * 4);
+                    dot[p] = dp4a((int)n[0], x.x, dot[p]);
+                    dot[p] = dp4a((int)n[1], x.y, dot[p]);
+                    dot[p] = dp4a((int)n[2], x.z, dot[p]);
+                    dot[p] = dp4a((int)n[3], x.w, dot[p]);
+                }
+            }
+            sum = fmaf(__half2float(s[b]) * __uint_as_float(hp[b * FX_WORDS + 24]), fix_value(dot), sum);
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        return sum;
+    }
+};
 
 // Barrier of a cooperatively launched grid, used once: *bar counts up from 0. The wait is
 // bounded (2^24 polls, the later ones 32 ns apart: about half a second); when it runs out
@@ -406,9 +493,84 @@ PI_DEV void exact_logits(const float* x, const float* router, const float* bias,
     __syncthreads();
 }
 
+struct FewRouting {  // in shared memory: [T][k], [T][k], [T]
+    const int* idx;
+    const float *gate, *share;
+};
+
+// The barrier and what follows it: the CTA's share of the (token, eight columns) units, token by
+// token, a warp to each expert's part of a unit. A warp's first weights are in its registers
+// before the barrier, each next one's on their way while one is worked on.
+template <int BPQ>
+PI_DEV void down_phase(const FewExpertArgs& a, const int d, const FewRouting& r, uint32_t* s_h, float* s_part,
+                       int* s_ok) {
+    constexpr int f = 128 * BPQ, hp = 4 * BPQ * FX_WORDS + (BPQ == 1 ? 0 : 16);  // hp: words of an expert's h
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int T = a.T, k = a.k, slots = k + a.has_shared, per_tok = d / 8;
+    const int64_t all = (int64_t)T * per_tok;
+    const int ub = (int)(all * blockIdx.x / gridDim.x), ue = (int)(all * (blockIdx.x + 1) / gridDim.x);
+    DownRows<BPQ> cur, nxt;
+    // part i of a pass: expert j = i % slots of its unit v = i / slots
+    auto load = [&](DownRows<BPQ>& to, int t, int col0, int v, int j) {
+        const int c = col0 + v * 8;
+        if (j == k) {
+            to.load(a.dns + c * (f / 2), a.dsd + c * (f / 32), lane);
+        } else {
+            const int64_t row = (int64_t)r.idx[t * k + j] * d + c;
+            to.load(a.dn + row * (f / 2), a.dd + row * (f / 32), lane);
+        }
+    };
+    const int v0 = warp / slots, j0 = warp - v0 * slots, dv = FE_W / slots, dj = FE_W - dv * slots;
+    auto pass = [&](int u) {  // units of one token that are summed together, a thread for each column
+        return min(min(FE_PART / slots, FE_T / 8), min(ue, (u / per_tok + 1) * per_tok) - u);
+    };
+    if (ub < ue && warp < pass(ub) * slots) load(cur, ub / per_tok, ub % per_tok * 8, v0, j0);
+    float residual = a.residual && ub < ue && tid < pass(ub) * 8 ? a.x[(int64_t)ub * 8 + tid] : 0.0f;
+    if (!grid_barrier(a.bar, a.err, s_ok)) return;
+    for (int u = ub, tok = -1; u < ue;) {
+        const int t = u / per_tok, n = pass(u), col0 = (u - t * per_tok) * 8;
+        if (t != tok) {
+            const float* ht = a.h + (int64_t)t * slots * f;
+            for (int i0 = 0; i0 < slots * (f / 4); i0 += FE_T) {  // whole warps: eight lanes make a block
+                const int i = min(i0 + tid, slots * (f / 4) - 1), j = i / (f / 4), b = (i & (f / 4 - 1)) >> 3;
+                fix_block(__ldcg(reinterpret_cast<const float4*>(ht) + i),
+                          s_h + j * hp + (b / BPQ) * h_quarter(BPQ) + (b % BPQ) * FX_WORDS, i & 7,
+                          i0 + tid < slots * (f / 4));
+            }
+            tok = t;
+            __syncthreads();
+        }
+        if (u != ub && warp < n * slots) load(cur, t, col0, v0, j0);
+        if (u != ub && a.residual && tid < n * 8) residual = a.x[(int64_t)u * 8 + tid];
+        for (int i = warp, v = v0, j = j0; i < n * slots; i += FE_W) {
+            const int now = j;
+            v += dv;
+            j += dj;
+            if (j >= slots) {
+                j -= slots;
+                ++v;
+            }
+            if (i + FE_W < n * slots) load(nxt, t, col0, v, j);
+            const float s = cur.sum(s_h + now * hp, lane);
+            if ((lane & 3) == 0) s_part[i * 8 + (lane >> 2)] = s;
+            cur = nxt;
+        }
+        __syncthreads();
+        if (tid < n * 8) {  // model/mod.rs:1525-1534, :1627-1633
+            const float* p = s_part + (tid >> 3) * slots * 8 + (tid & 7);
+            float acc = 0.0f;
+            for (int j = 0; j < k; ++j) acc = fadd(acc, fmul(r.gate[t * k + j], p[j * 8]));
+            if (a.has_shared) acc = fadd(acc, fmul(r.share[t], p[k * 8]));
+            a.out[(int64_t)u * 8 + tid] = a.residual ? fadd(residual, acc) : acc;
+        }
+        __syncthreads();
+        u += n;
+    }
+}
+
 template <int CPL, int NPL>
 __global__ __launch_bounds__(FE_T, 1) void k_few_experts(const FewExpertArgs a) {
-    extern __shared__ __align__(16) float s_dyn[];  // gate/up: inputs of the group's tokens; down: h
+    extern __shared__ __align__(16) uint32_t s_dyn[];  // gate/up: inputs of the group's tokens; down: h
     __shared__ int s_idx[FEW_T * 32], s_use[FE_ITEMS], s_mask[FE_T], s_item[FE_ITEMS], s_count[FE_W], s_nuse, s_ok;
     __shared__ uint32_t s_open;
     __shared__ float s_gate[FEW_T * 32], s_share[FEW_T], s_inv, s_part[FE_PART * 8];
@@ -418,13 +580,11 @@ __global__ __launch_bounds__(FE_T, 1) void k_few_experts(const FewExpertArgs a) 
     const int grp = blockIdx.x % a.n_groups, t0 = grp * a.group, nt = min(a.group, T - t0);
     const int cta = blockIdx.x / a.n_groups, n_cta = (gridDim.x - grp + a.n_groups - 1) / a.n_groups;
 
-    // the group's inputs, 36 floats a block
-    for (int i = tid; i < nt * (d / 4); i += FE_T) {
-        const int t = i / (d / 4), c = i - t * (d / 4);
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(
-                         s_dyn + (t * nb + (c >> 3)) * 36 + (c & 7) * 4)),
-                     "l"(a.xin + (int64_t)(t0 + t) * d + 4 * c)
-                     : "memory");
+    {  // the group's inputs
+        const uint32_t to = (uint32_t)__cvta_generic_to_shared(s_dyn);
+        const uint32_t* from = a.xfix + (int64_t)t0 * nb * FX_WORDS;
+        for (int i = tid; i < nt * nb * (FX_WORDS / 4); i += FE_T)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + i * 16), "l"(from + i * 4) : "memory");
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
     // routing of every token (a warp each), in every CTA
@@ -445,27 +605,6 @@ __global__ __launch_bounds__(FE_T, 1) void k_few_experts(const FewExpertArgs a) 
             topk_token<NPL, true>(s_part, 0, E, k, a.has_shgate, s_idx + t * k, s_gate + t * k, s_share + t, nullptr,
                                   s_part + FE_MAXE, s_item, lane);
         __syncthreads();
-    }
-    // What this CTA's part of the down projection will read goes to L2 meanwhile (T = 1: the
-    // phase behind the barrier took 4.7 us, most of it the first trip to memory).
-    const int per_tok = d / 8, bpq = f / 128, hp = f + 16;  // hp: floats of a padded h row
-    const int64_t all = (int64_t)T * per_tok;
-    const int ub = (int)(all * blockIdx.x / gridDim.x), ue = (int)(all * (blockIdx.x + 1) / gridDim.x);
-    {
-        const int lines = f / 32 + max(1, f / 256);  // 128-byte lines of eight rows: 4 f of nibbles, f / 2 of scales
-        const int v0 = ub + warp / 2;                // 16 lanes take the pieces of a unit
-        for (int v = v0; v < ue; v += FE_W / 2) {
-            const int t = v / per_tok, c0 = (v - t * per_tok) * 8;
-            for (int j = 0; j < slots; ++j) {
-                const int e = j < k ? s_idx[t * k + j] : E;
-                const int64_t row = (e == E ? 0 : (int64_t)e * d) + c0;
-                const uint8_t* D = (e == E ? a.dns : a.dn) + row * (f / 2);
-                const uint8_t* DD = reinterpret_cast<const uint8_t*>((e == E ? a.dsd : a.dd) + row * (f / 32));
-                const int l = (warp & 1) * 32 + lane;
-                if (l < lines)
-                    asm volatile("prefetch.global.L2 [%0];" ::"l"(l < f / 32 ? D + l * 128 : DD + (l - f / 32) * 128));
-            }
-        }
     }
     // The group's work: items of an expert and up to four of its tokens, which share the decoded
     // weights. The shared expert's come first, then those of several tokens, so that the
@@ -513,16 +652,27 @@ __global__ __launch_bounds__(FE_T, 1) void k_few_experts(const FewExpertArgs a) 
     __syncthreads();
 
     // gate, up and SwiGLU: a warp takes two rows of an expert for the tokens of an item
-    const int half_f = f / 2, n_unit = s_nuse * half_f;
-    for (int unit = cta * FE_W + warp; unit < n_unit; unit += n_cta * FE_W) {
-        const int item = unit / half_f, e = s_use[item], row = 2 * (unit - item * half_f);
-        const bool sh = e == E;
+    const int half_f = f / 2, lf = 31 - __clz(half_f), n_unit = s_nuse * half_f, stride = n_cta * FE_W;
+    auto rows = [&](int unit) {
+        const int e = s_use[unit >> lf], r = 2 * (unit & (half_f - 1));
+        if (e == E)
+            return RowPtrs{a.gs + r * (d / 2), a.us + r * (d / 2), a.gsd + r * nb, a.usd + r * nb};
+        const int64_t q = (int64_t)(e * f + r);  // E f < 2^20
+        return RowPtrs{a.g + q * (d / 2), a.u + q * (d / 2), a.gd + q * nb, a.ud + q * nb};
+    };
+    RowChunk chunk;
+    RowPtrs at = {}, next = {};
+    const int first = cta * FE_W + warp;
+    if (first < n_unit) {
+        at = rows(first);
+        chunk.load(at, nb, lane);
+    }
+    for (int unit = first; unit < n_unit; unit += stride) {
+        const int item = unit >> lf, e = s_use[item], row = 2 * (unit & (half_f - 1));
         uint32_t mask = s_item[item];
-        const int64_t r = (sh ? 0 : (int64_t)e * f) + row;
-        const uint8_t *G = (sh ? a.gs : a.g) + r * (d / 2), *U = (sh ? a.us : a.u) + r * (d / 2);
-        const __half *GD = (sh ? a.gsd : a.gd) + r * nb, *UD = (sh ? a.usd : a.ud) + r * nb;
+        next = unit + stride < n_unit ? rows(unit + stride) : at;  // the last one reads its own first chunk again
         int tok[FE_TB], n = 0;
-        const float* xs[FE_TB];
+        const uint32_t* xs[FE_TB];
 #pragma unroll
         for (int i = 0; i < FE_TB; ++i) {  // an item that is not full repeats its last token
             if (mask) {
@@ -532,80 +682,35 @@ __global__ __launch_bounds__(FE_T, 1) void k_few_experts(const FewExpertArgs a) 
             } else {
                 tok[i] = tok[i > 0 ? i - 1 : 0];
             }
-            xs[i] = s_dyn + tok[i] * nb * 36;
+            xs[i] = s_dyn + tok[i] * nb * FX_WORDS;
         }
-        float sum[4][FE_TB];
+        float sum[FE_TB];
         if (n == 1) {
-            float s1[4][1];
-            const float* const x1[1] = {xs[0]};
-            gateup_rows<CPL, 1>(G, U, GD, UD, d, x1, lane, s1);
-#pragma unroll
-            for (int v = 0; v < 4; ++v) sum[v][0] = s1[v][0];
+            const uint32_t* const x1[1] = {xs[0]};
+            gateup_rows<CPL, 1>(chunk, at, next, x1, lane, sum);
         } else if (n == 2) {
-            float s2[4][2];
-            const float* const x2[2] = {xs[0], xs[1]};
-            gateup_rows<CPL, 2>(G, U, GD, UD, d, x2, lane, s2);
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                sum[v][0] = s2[v][0];
-                sum[v][1] = s2[v][1];
-            }
+            const uint32_t* const x2[2] = {xs[0], xs[1]};
+            gateup_rows<CPL, 2>(chunk, at, next, x2, lane, sum);
         } else {
-            gateup_rows<CPL, FE_TB>(G, U, GD, UD, d, xs, lane, sum);
+            gateup_rows<CPL, FE_TB>(chunk, at, next, xs, lane, sum);
         }
 #pragma unroll
         for (int i = 0; i < FE_TB; ++i) {
             if (i >= n) break;
             const int t = t0 + tok[i];
             int j = k;
-            if (!sh) j = __ffs(__ballot_sync(0xffffffffu, lane < k && s_idx[t * k + lane] == e)) - 1;
-            if (lane < 2)
-                a.h[((int64_t)t * slots + j) * f + row + lane] =
-                    swiglu_ref(lane ? sum[2][i] : sum[0][i], lane ? sum[3][i] : sum[1][i]);
+            if (e != E) j = __ffs(__ballot_sync(0xffffffffu, lane < k && s_idx[t * k + lane] == e)) - 1;
+            const float g = sum[i], u = __shfl_down_sync(0xffffffffu, g, 8);
+            if ((lane & 15) == 0) a.h[((int64_t)t * slots + j) * f + row + (lane >> 4)] = g / (1.0f + expf(-g)) * u;
         }
+        at = next;
     }
-    if (!grid_barrier(a.bar, a.err, &s_ok)) return;
-
-    // down: the CTA's share of the (token, eight columns) units, token by token
-    for (int u = ub; u < ue;) {
-        const int t = u / per_tok, tok_end = min(ue, (t + 1) * per_tok);
-        __syncthreads();
-        for (int i = tid; i < slots * (f / 4); i += FE_T) {
-            const int j = i / (f / 4), c = 4 * (i - j * (f / 4)), q = c / (f / 4);
-            *reinterpret_cast<float4*>(s_dyn + j * hp + c + 4 * q) =
-                __ldcg(reinterpret_cast<const float4*>(a.h + ((int64_t)t * slots + j) * f + c));
-        }
-        __syncthreads();
-        while (u < tok_end) {
-            const int n = min(FE_PART / slots, tok_end - u), col0 = (u - t * per_tok) * 8;
-            for (int i = warp; i < n * slots; i += FE_W) {
-                const int v = i / slots, j = i - v * slots;
-                const int e = j < k ? s_idx[t * k + j] : E;
-                const int64_t row = (e == E ? 0 : (int64_t)e * d) + col0 + v * 8;
-                const uint8_t* D = (e == E ? a.dns : a.dn) + row * (f / 2);
-                const __half* DD = (e == E ? a.dsd : a.dd) + row * (f / 32);
-                const float* hs = s_dyn + j * hp;
-                float s;
-                switch (bpq) {
-                    case 1: s = down_rows<1>(D, DD, hs, lane); break;
-                    case 2: s = down_rows<2>(D, DD, hs, lane); break;
-                    case 4: s = down_rows<4>(D, DD, hs, lane); break;
-                    default: s = down_rows<8>(D, DD, hs, lane); break;
-                }
-                if ((lane & 3) == 0) s_part[(v * slots + j) * 8 + (lane >> 2)] = s;
-            }
-            __syncthreads();
-            for (int i = tid; i < n * 8; i += FE_T) {  // model/mod.rs:1525-1534, :1627-1633
-                const float* p = s_part + (i >> 3) * slots * 8 + (i & 7);
-                float acc = 0.0f;
-                for (int j = 0; j < k; ++j) acc = fadd(acc, fmul(s_gate[t * k + j], p[j * 8]));
-                if (a.has_shared) acc = fadd(acc, fmul(s_share[t], p[k * 8]));
-                const int64_t o = (int64_t)t * d + col0 + i;
-                a.out[o] = a.residual ? fadd(a.x[o], acc) : acc;
-            }
-            __syncthreads();
-            u += n;
-        }
+    const FewRouting routing{s_idx, s_gate, s_share};
+    switch (f / 128) {
+        case 1: down_phase<1>(a, d, routing, s_dyn, s_part, &s_ok); break;
+        case 2: down_phase<2>(a, d, routing, s_dyn, s_part, &s_ok); break;
+        case 4: down_phase<4>(a, d, routing, s_dyn, s_part, &s_ok); break;
+        default: down_phase<8>(a, d, routing, s_dyn, s_part, &s_ok); break;
     }
 }
 
@@ -615,8 +720,8 @@ __global__ __launch_bounds__(FE_T, 1) void k_few_experts(const FewExpertArgs a) 
 constexpr size_t FEW_X_BYTES = 180 * 1024;  // inputs of the tokens a CTA keeps for gate/up
 
 struct FewBufs {
-    float *logits, *eps, *normed, *h;
-    uint32_t* bar;
+    float *logits, *eps, *h;
+    uint32_t *xfix, *bar;
     size_t bytes;
 };
 FewBufs few_carve(const pi_moe_layer* L, int64_t T, char* base) {
@@ -625,7 +730,7 @@ FewBufs few_carve(const pi_moe_layer* L, int64_t T, char* base) {
     o.bar = b.take<uint32_t>(1);
     o.logits = b.take<float>(T * (L->E + 1));
     o.eps = b.take<float>(T * (L->E + 1));
-    o.normed = b.take<float>(T * L->d);
+    o.xfix = b.take<uint32_t>(T * (L->d / 32) * FX_WORDS);
     o.h = b.take<float>(T * (L->k + (L->has_shared ? 1 : 0)) * L->f);
     o.bytes = b.off + 256;
     return o;
@@ -633,8 +738,8 @@ FewBufs few_carve(const pi_moe_layer* L, int64_t T, char* base) {
 
 template <int CPL, int NPL>
 cudaError_t launch_experts(const FewExpertArgs& a, int sms, cudaStream_t st) {
-    const size_t x = (size_t)a.group * (a.d / 32) * 36 * 4;
-    const size_t h = (size_t)(a.k + a.has_shared) * (a.f + 16) * 4, smem = std::max(x, h);
+    const size_t x = (size_t)a.group * (a.d / 32) * FX_WORDS * 4;
+    const size_t h = (size_t)(a.k + a.has_shared) * (a.f / 32 * FX_WORDS + 16) * 4, smem = std::max(x, h);
     auto kern = k_few_experts<CPL, NPL>;
     // the limit is always raised: beside the kernel's 26 KB of static shared memory the default
     // of 48 KB would not hold what pi_smem_attr lets pass as small
@@ -682,12 +787,12 @@ int few_forward(pi_ctx* ctx, const pi_moe_layer* L, const float* x, int64_t T, f
         const int R = (int)std::min<int64_t>(fit, std::max<int64_t>(2, ((E + 1) * groups + sms - 1) / sms));
         const size_t smem = row * (FL_GROUP + R);
         pi_smem_attr((const void*)k_few_logits, smem);
-        const FewLogitArgs a{x, L->router, L->bias, (int)T, d, E, R, norm ? 1 : 0, B.normed, B.logits, B.eps, B.bar};
+        const FewLogitArgs a{x, L->router, L->bias, (int)T, d, E, R, norm ? 1 : 0, B.logits, B.eps, B.xfix, B.bar};
         pi_pdl_launch(k_few_logits, dim3((unsigned)((E + R) / R), (unsigned)groups), dim3(FL_T), smem, st, a);
         if (int rc = pi_cuda_check(ctx, cudaGetLastError(), "moe fused logits")) return rc;
     }
     PiProfScope ps(ctx, st, "k_few_experts");
-    const int group = (int)std::min<int64_t>(T, (int64_t)(FEW_X_BYTES / (d / 32 * 36 * 4)));
+    const int group = (int)std::min<int64_t>(T, (int64_t)(FEW_X_BYTES / (d / 32 * FX_WORDS * 4)));
     FewExpertArgs a = {};
     a.g = (const uint8_t*)L->gate.q;
     a.u = (const uint8_t*)L->up.q;
@@ -704,7 +809,7 @@ int few_forward(pi_ctx* ctx, const pi_moe_layer* L, const float* x, int64_t T, f
         a.dsd = L->down_sh.d;
     }
     a.x = x;
-    a.xin = norm ? B.normed : x;
+    a.xfix = B.xfix;
     a.logits = B.logits;
     a.eps = B.eps;
     a.router = L->router;

@@ -1,11 +1,15 @@
 """The MoE layer of a few tokens in two kernels (``path="fused"``), against the definition in 64
 bits over the reference's own routing, and against the layer's other path.
 
-Tolerance, u = 2^-24, from the kernels' own sums: a gate or up sum adds 32 products a block (two
-partial sums of 16), a scale, its lane's blocks and five shuffles: at most 16 + 2 + 4 + 5 + 1 = 28
-roundings of its absolute terms; a down sum 16 + 2 + 8 + 2 + 1 = 29. h = g s(g) u moves by
-1.1 |u| dg + |g s(g)| du and rounds four times. Gates are the reference's (bit-exact routing); the
-shared expert's gate is a sequential sum of d terms through a sigmoid (slope 1/4)."""
+Tolerance, u = 2^-24, from the kernels' own sums. 32 inputs become integers of at least 2^21 for the
+largest: each is within 2^-22 of the block's largest, F = 2^-22 max|block|. Block dots are exact
+integers, turned into f32 with 3 roundings, scaled with 1 and added with 1; then a lane's blocks
+(4 at most, 8 in a down row) and five (two) shuffles: at most 5 + 4 + 5 = 14 and 5 + 8 + 2 = 15
+roundings of a block's absolute terms, which are at most (|x| + F) |w|. RMSNorm's input is the
+reference's up to d / 8 + 64 roundings of one common factor (its sum of squares is sequential).
+h = g s(g) u moves by 1.1 |u| dg + |g s(g)| du and rounds five times. Gates: logits are sums of 32
+segments, within (d / 32 + 8) u sum|p| of exact ones, the reference's sequential ones within d u
+sum|p|; a gate moves by twice the largest such change, relatively."""
 import numpy as np
 import pytest
 
@@ -31,34 +35,43 @@ def _make(w, d, f, E, k):
                         router_bias=w["bias"])
 
 
-def _expert(orc, gate, up, down, d, f, x):
-    """(y, bound of its error) of one expert for one token, in 64 bits."""
+def _fix(v):
+    """What fixed point may move each value by: 2^-22 of its block's largest."""
+    return np.repeat(np.abs(v).reshape(-1, 32).max(1), 32) * 2.0 ** -22
+
+
+def _expert(orc, gate, up, down, d, f, x, dx):
+    """(y, bound of its error) of one expert for one token, in 64 bits; dx: what is known of x."""
     deq = lambda r, n, m: np.asarray(orc.dequantize(r, 2, n, m), np.float64).reshape(n, m)  # noqa: E731
     G, Up, D = deq(gate, f, d), deq(up, f, d), deq(down, d, f)
     g, u = G @ x, Up @ x
-    dg, du = 28 * U * (np.abs(G) @ np.abs(x)), 28 * U * (np.abs(Up) @ np.abs(x))
+    e = dx + _fix(x) + 14 * U * np.abs(x)
+    dg, du = np.abs(G) @ e, np.abs(Up) @ e
     s = g / (1 + np.exp(-g))
     h, dh = s * u, 1.1 * np.abs(u) * dg + np.abs(s) * du + 5 * U * np.abs(s * u)
-    return D @ h, np.abs(D) @ dh + 29 * U * (np.abs(D) @ np.abs(h))
+    return D @ h, np.abs(D) @ (1.01 * dh + 1.01 * _fix(h) + 15 * U * np.abs(h))
 
 
 def _reference(orc, w, x, d, f, E, k, norm, residual):
-    T, b = x.shape[0], d // 32 * 18
+    T = x.shape[0]
     xin = np.stack([orc.rms_norm(r, np.ones(d, np.float32)) for r in x]) if norm else x
     r = orc.moe_route(xin, w["router"], d, E, k, bias=w["bias"])
     out, tol = np.zeros((T, d)), np.zeros((T, d))
     cut = lambda a, e: a.reshape(E, -1)[e]  # noqa: E731
+    router = np.abs(w["router"].reshape(E, d)).astype(np.float64)
     for t in range(T):
         xt = xin[t].astype(np.float64)
+        dx = (d / 8 + 66) * U * np.abs(xt) if norm else np.zeros(d)
+        moved = 2 * (d + d / 32 + 8 + (d / 8 + 66) * norm + 4) * U * (router[r["idx"][t]] @ np.abs(xt)).max()
         terms = []
         for e, g in zip(r["idx"][t], r["gates"][t]):
-            y, dy = _expert(orc, cut(w["gate"], e), cut(w["up"], e), cut(w["down"], e), d, f, xt)
-            terms.append((float(g), 0.0, y, dy))
+            y, dy = _expert(orc, cut(w["gate"], e), cut(w["up"], e), cut(w["down"], e), d, f, xt, dx)
+            terms.append((float(g), float(g) * (moved + (k + 8) * U), y, dy))
         if w["shared"]:
             gate, up, down, sg = w["shared"]
-            y, dy = _expert(orc, gate, up, down, d, f, xt)
+            y, dy = _expert(orc, gate, up, down, d, f, xt, dx)
             z = 0.0 if sg is None else sg.astype(np.float64) @ xt
-            dz = 0.0 if sg is None else (d + 8) * U * (np.abs(sg) @ np.abs(xt))
+            dz = 0.0 if sg is None else (d / 32 + 8 + (d / 8 + 66) * norm) * U * (np.abs(sg) @ np.abs(xt))
             terms.append((1.0 if sg is None else 1 / (1 + np.exp(-z)), dz / 4 + 4 * U, y, dy))
         for g, dgate, y, dy in terms:
             out[t] += g * y
