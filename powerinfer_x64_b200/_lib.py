@@ -196,6 +196,13 @@ def stream_ptr(stream=None):
     return _P(stream.cuda_stream) if hasattr(stream, "cuda_stream") else _P(stream)
 
 
+def raw_stream(device: int) -> int:
+    """cudaStream_t of torch's current stream on ``device`` (without making a Stream object)."""
+    import torch
+
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
 def ptr(t) -> _P:
     """Device pointer of a torch tensor (None -> NULL)."""
     if t is None:

@@ -10,7 +10,7 @@ from typing import Any, NamedTuple
 
 import torch
 
-from ._lib import PI_ERR_ARG, PI_QT_BF16, PI_QT_F16, PI_QT_F32, Context, PiError, lib
+from ._lib import PI_ERR_ARG, PI_QT_BF16, PI_QT_F16, PI_QT_F32, Context, PiError, lib, raw_stream
 
 _DTYPES = {torch.float32: PI_QT_F32, torch.float16: PI_QT_F16, torch.bfloat16: PI_QT_BF16}
 
@@ -35,10 +35,11 @@ def token_logprobs(logits, targets=None, n_top: int = 0) -> TokenLogprobs:
     A logit of -inf masks its token. A row that is all -inf has entropy 0, log
     probabilities -inf and ids -1; a row with a NaN or +inf gives NaN and ids -1.
     """
-    if not logits.is_cuda or logits.dim() != 2 or logits.dtype not in _DTYPES:
+    qt = _DTYPES.get(logits.dtype)
+    if qt is None or logits.dim() != 2 or not logits.is_cuda:
         raise PiError(PI_ERR_ARG, "logprobs: logits must be a CUDA tensor [T, V] of f32, f16 or bf16")
-    T, V = logits.shape
-    if V < 1 or (V > 1 and logits.stride(1) != 1):
+    (T, V), (ld, step) = logits.shape, logits.stride()
+    if V < 1 or (V > 1 and step != 1):
         raise PiError(PI_ERR_ARG, "logprobs: need V >= 1 logits a row, next to one another")
     dev, K, logp = logits.device, 0, None
     if targets is not None:
@@ -47,7 +48,7 @@ def token_logprobs(logits, targets=None, n_top: int = 0) -> TokenLogprobs:
             raise PiError(PI_ERR_ARG, "logprobs: targets must be int64 [T] or [T, K] on the logits' device")
         targets = targets.contiguous()
         K = 1 if targets.dim() == 1 else targets.shape[1]
-        logp = torch.empty(targets.shape, dtype=torch.float32, device=dev)
+        logp = torch.empty_like(targets, dtype=torch.float32)
     entropy = torch.empty(T, dtype=torch.float32, device=dev)
     ids = top = None
     if n_top:
@@ -57,9 +58,10 @@ def token_logprobs(logits, targets=None, n_top: int = 0) -> TokenLogprobs:
         top = torch.empty((T, n_top), dtype=torch.float32, device=dev)
     if T:
         ctx = Context.of(dev.index)
-        ctx.check(lib().pi_token_logprobs(ctx.h, logits.data_ptr(), _DTYPES[logits.dtype], T, V, logits.stride(0),
-                                          targets.data_ptr() if K else None, K, n_top,
-                                          logp.data_ptr() if K else None, entropy.data_ptr(),
-                                          ids.data_ptr() if n_top else None, top.data_ptr() if n_top else None,
-                                          torch.cuda.current_stream(dev).cuda_stream))
+        rc = lib().pi_token_logprobs(ctx.h, logits.data_ptr(), qt, T, V, ld, targets.data_ptr() if K else None, K,
+                                     n_top, logp.data_ptr() if K else None, entropy.data_ptr(),
+                                     ids.data_ptr() if n_top else None, top.data_ptr() if n_top else None,
+                                     raw_stream(dev.index))
+        if rc:
+            ctx.check(rc)
     return TokenLogprobs(logp, entropy, ids, top)

@@ -15,7 +15,7 @@ import numpy as np
 import torch
 
 from ._lib import (PI_ERR_ARG, PI_ERR_INDEX, PI_QT_BF16, PI_QT_F16, PI_QT_F32, Context,
-                   PiError, PiLoraBank, lib)
+                   PiError, PiLoraBank, lib, raw_stream)
 
 _DTYPES = {torch.float32: PI_QT_F32, torch.float16: PI_QT_F16, torch.bfloat16: PI_QT_BF16}
 
@@ -69,7 +69,7 @@ class SharedProjection:
         on_dev = hasattr(raw, "is_cuda") and raw.is_cuda
         if device is None:
             device = raw.device.index if on_dev else torch.cuda.current_device()
-        self.device = torch.device("cuda", device)
+        self.device, self.index, self._ws_bytes = torch.device("cuda", device), device, {}
         self.ctx = Context.of(device)
         if on_dev:
             if raw.device != self.device or raw.dtype != torch.uint8 or not raw.is_contiguous():
@@ -97,30 +97,36 @@ class SharedProjection:
 
         adapter_ids: int32 [T], the adapter of each token, negative for none; an id past the
         bank adds nothing and is reported by ``Context.sync_check`` (PI_ERR_INDEX)."""
-        dev = self.device
-        if x.dtype != torch.float32 or x.device != dev or x.dim() != 2 or x.shape[1] != self.n_in or \
+        dev, n_in, n_out = self.index, self.n_in, self.n_out
+        if x.dtype != torch.float32 or x.get_device() != dev or x.dim() != 2 or x.shape[1] != n_in or \
                 not x.is_contiguous():
-            raise PiError(PI_ERR_ARG, f"projection: x must be contiguous f32 [T, {self.n_in}] on {dev}")
+            raise PiError(PI_ERR_ARG, f"projection: x must be contiguous f32 [T, {n_in}] on {self.device}")
         T = x.shape[0]
         if (bank is None) != (adapter_ids is None):
             raise PiError(PI_ERR_ARG, "projection: a bank and adapter_ids come together")
+        desc, ids, rank = None, None, 0
         if bank is not None:
-            if bank.n_in != self.n_in or bank.n_out != self.n_out or bank.device != dev:
+            if bank.n_in != n_in or bank.n_out != n_out or bank.device != self.device:
                 raise PiError(PI_ERR_ARG, f"projection: the bank is for [{bank.n_out}][{bank.n_in}] on {bank.device}")
-            if adapter_ids.dtype != torch.int32 or adapter_ids.shape != (T,) or adapter_ids.device != dev or \
+            if adapter_ids.dtype != torch.int32 or adapter_ids.shape != (T,) or adapter_ids.get_device() != dev or \
                     not adapter_ids.is_contiguous():
-                raise PiError(PI_ERR_ARG, f"projection: adapter_ids must be contiguous int32 [T] on {dev}")
+                raise PiError(PI_ERR_ARG, f"projection: adapter_ids must be contiguous int32 [T] on {self.device}")
+            desc, ids, rank = bank._desc, adapter_ids.data_ptr(), bank.rank
         if out is None:
-            out = torch.empty((T, self.n_out), dtype=torch.float32, device=dev)
-        elif out.dtype != torch.float32 or out.shape != (T, self.n_out) or out.device != dev or \
+            out = torch.empty((T, n_out), dtype=torch.float32, device=self.device)
+        elif out.dtype != torch.float32 or out.shape != (T, n_out) or out.get_device() != dev or \
                 not out.is_contiguous():
-            raise PiError(PI_ERR_ARG, f"projection: out must be contiguous f32 [T, {self.n_out}] on {dev}")
+            raise PiError(PI_ERR_ARG, f"projection: out must be contiguous f32 [T, {n_out}] on {self.device}")
         if T == 0:
             return out
-        L, desc = lib(), None if bank is None else bank._desc
-        nbytes = L.pi_proj_workspace(self.h, T, desc)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)  # the caching allocator's: one per call and graph
-        self.ctx.check(L.pi_proj_forward(self.ctx.h, self.h, x.data_ptr(), T, desc,
-                                         None if bank is None else adapter_ids.data_ptr(), out.data_ptr(),
-                                         ws.data_ptr(), nbytes, torch.cuda.current_stream(dev).cuda_stream))
+        L = lib()
+        nbytes = self._ws_bytes.get((T, rank))
+        if nbytes is None:
+            nbytes = self._ws_bytes[(T, rank)] = L.pi_proj_workspace(self.h, T, desc)
+        # the caching allocator's memory: one workspace per call and per captured graph
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        rc = L.pi_proj_forward(self.ctx.h, self.h, x.data_ptr(), T, desc, ids, out.data_ptr(), ws.data_ptr(), nbytes,
+                               raw_stream(dev))
+        if rc:
+            self.ctx.check(rc)
         return out

@@ -18,7 +18,7 @@ import numpy as np
 
 from . import quant
 from ._lib import (PI_FWD_FAST_SUM, PI_FWD_FORCE_GEMM, PI_FWD_FORCE_GEMV, PI_FWD_RESIDUAL, PI_FWD_RMSNORM, PI_QT_F32, Context, PiError, PiMoeLayerDesc, PI_ERR_ARG, lib,
-                   ptr, stream_ptr)
+                   ptr, raw_stream, stream_ptr)
 
 
 def _torch():
@@ -67,7 +67,7 @@ class MoeLayer:
         h = C.c_void_p()
         torch.cuda.synchronize()
         self.ctx.check(lib().pi_moe_layer_create(self.ctx.h, C.byref(desc), C.byref(h)))
-        self.h = h
+        self.h, self._fused_ws = h, {}
 
     def __del__(self):
         try:
@@ -123,24 +123,30 @@ class MoeLayer:
         torch = _torch()
         if fast:
             raise PiError(PI_ERR_ARG, "moe: the fused path has no fast sum")
-        dev = torch.device("cuda", self.ctx.device)
-        x = quant._f32(x)
-        if x.dtype != torch.float32 or x.device != dev or not x.is_contiguous() or x.numel() % self.n_embd:
-            raise PiError(PI_ERR_ARG, f"moe: x must be contiguous f32 [T, {self.n_embd}] on {dev}")
-        T = x.numel() // self.n_embd
+        x, dev, d = quant._f32(x), self.ctx.device, self.n_embd
+        n = x.numel()
+        if x.dtype != torch.float32 or x.get_device() != dev or not x.is_contiguous() or n % d:
+            raise PiError(PI_ERR_ARG, f"moe: x must be contiguous f32 [T, {d}] on cuda:{dev}")
+        T = n // d
         if out is None:
-            out = torch.empty((T, self.n_embd), dtype=torch.float32, device=dev)
-        elif out.dtype != torch.float32 or out.device != dev or not out.is_contiguous() or \
-                out.numel() != x.numel():
-            raise PiError(PI_ERR_ARG, f"moe: out must be contiguous f32 [T, {self.n_embd}] on {dev}")
+            out = torch.empty((T, d), dtype=torch.float32, device=x.device)
+        elif out.dtype != torch.float32 or out.get_device() != dev or not out.is_contiguous() or out.numel() != n:
+            raise PiError(PI_ERR_ARG, f"moe: out must be contiguous f32 [T, {d}] on cuda:{dev}")
         L, flags = lib(), (PI_FWD_RMSNORM if rmsnorm else 0) | (PI_FWD_RESIDUAL if residual else 0)
-        nbytes = L.pi_moe_fused_workspace(self.h, T)
-        s = torch.cuda.current_stream(dev) if stream is None else stream
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)  # the caching allocator's: one per call and graph
-        if stream is not None:
-            ws.record_stream(s)
-        self.ctx.check(L.pi_moe_forward_fused(self.ctx.h, self.h, x.data_ptr(), T, out.data_ptr(), flags,
-                                              ws.data_ptr() if nbytes else None, nbytes, s.cuda_stream))
+        nbytes = self._fused_ws.get(T)
+        if nbytes is None:
+            nbytes = self._fused_ws[T] = L.pi_moe_fused_workspace(self.h, T)
+        # the caching allocator's memory: one workspace per call and per captured graph
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        if stream is None:
+            raw = raw_stream(dev)
+        else:
+            raw = stream.cuda_stream
+            ws.record_stream(stream)
+        rc = L.pi_moe_forward_fused(self.ctx.h, self.h, x.data_ptr(), T, out.data_ptr(), flags,
+                                    ws.data_ptr() if nbytes else None, nbytes, raw)
+        if rc:
+            self.ctx.check(rc)
         return out
 
     def forward_routed(self, x, out=None, rmsnorm: bool = False, residual: bool = False, stream=None,
