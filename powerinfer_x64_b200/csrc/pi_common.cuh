@@ -126,6 +126,11 @@ PI_DEV uint64_t add2(uint64_t a, uint64_t b) {
 PI_DEV void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 PI_DEV void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// Cluster barrier in two halves: what a CTA wrote (into another's shared memory too) before it
+// arrives is visible to those that have waited. A CTA that need not wait may exit instead.
+PI_DEV void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+PI_DEV void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 PI_DEV int4 ld_stream(const void* p) {
     int4 r;
     asm volatile("ld.global.nc.L1::no_allocate.v4.s32 {%0,%1,%2,%3}, [%4];"

@@ -29,6 +29,7 @@ namespace {
 constexpr int LP_NT = 256;       // threads of a CTA
 constexpr int LP_W = LP_NT / 32;
 constexpr int LP_U = 2;          // 16-byte loads of a step; the next step's are in flight
+constexpr int LP_OCC = 4;        // CTAs of an SM
 constexpr int LP_MAXC = 16;      // CTAs of a cluster at most
 constexpr int LP_MAXTOP = 32;    // alternatives at most
 constexpr float LP_LOG2E = 1.4426950408889634f;
@@ -207,11 +208,13 @@ PI_DEV void lp_join_lanes(LpStat& st, int width) {
 // least, so only what reaches it is kept from the start (about n values of the first
 // 2048 or 4096, then n / i of the i-th step), and the buffers hardly ever fill.
 template <typename ET, bool TOP>
-__global__ __launch_bounds__(LP_NT, 3) void k_token_logprobs(const LogprobArgs a) {
+__global__ __launch_bounds__(LP_NT, LP_OCC) void k_token_logprobs(const LogprobArgs a) {
     constexpr int NV = 16 / (int)sizeof(ET);
     constexpr int CAP = 64 + 32 * NV;  // n kept after compact() and one load of every lane
     __shared__ uint64_t s_buf[TOP ? LP_W * CAP : 1];
     __shared__ uint64_t s_all[TOP ? LP_MAXC * LP_MAXTOP : 1];
+    __shared__ uint64_t s_lists[TOP ? LP_MAXC * LP_MAXTOP : 1];  // the cluster's lists, in its first CTA
+    __shared__ LpStat s_stats[LP_MAXC];                          // and its states
     __shared__ uint64_t s_best[LP_MAXTOP];
     __shared__ LpStat s_stat[LP_W], s_cta;
     __shared__ float s_max[64], s_thr;
@@ -228,6 +231,8 @@ __global__ __launch_bounds__(LP_NT, 3) void k_token_logprobs(const LogprobArgs a
     const int4* xv = reinterpret_cast<const int4*>(x + head);
     const int64_t step = (int64_t)C * LP_NT;
     const bool edges = rank == 0 && warp == 0;
+    // the first CTA of the cluster must run before the others write into its shared memory
+    if (C > 1) cluster_arrive();
 
     LpStat st{LP_LOWEST, 0.0f, 0.0f};
     auto scalar = [&](float v) {
@@ -351,8 +356,8 @@ __global__ __launch_bounds__(LP_NT, 3) void k_token_logprobs(const LogprobArgs a
         __syncthreads();
         int total = 0;
         for (int i = 0; i < LP_W; ++i) total += s_cnt[i];
-        __syncthreads();
         if (total > LP_NT) {
+            __syncthreads();
             if (top.cnt > a.n_top) top.compact();
             if (lane == 0) s_cnt[warp] = top.cnt;
             __syncthreads();
@@ -375,39 +380,37 @@ __global__ __launch_bounds__(LP_NT, 3) void k_token_logprobs(const LogprobArgs a
         if (lane == 0) s_cta = t;
     }
     if (C > 1) {
+        __syncthreads();
+        cluster_wait();
         cg::cluster_group cl = cg::this_cluster();
-        cl.sync();
-        if (rank == 0) {
-            if (warp == 0) {
-                LpStat t = *cl.map_shared_rank(&s_cta, lane % C);
-                lp_join_lanes(t, C);
-                if (lane == 0) s_stat[0] = t;
-            }
-            if constexpr (TOP) {
-                // ceil(n / C) values of every CTA reach the least of the CTAs' ceil(n / C)-th
-                // ones, n values at least: only what reaches it is ranked
-                const int deep = (a.n_top + C - 1) / C;
-                uint64_t* lists = s_buf;  // done with: every warp has copied its keys
-                if (tid == 0) s_cnt[0] = 0;
-                for (int i = tid; i < C * a.n_top; i += LP_NT) {
-                    const int c = i / a.n_top;
-                    lists[i] = cl.map_shared_rank(s_best, c)[i - c * a.n_top];
-                }
-                __syncthreads();
-                uint64_t bound = ~0ull;
-                for (int c = 0; c < C; ++c) {
-                    const uint64_t k = lists[c * a.n_top + deep - 1];
-                    bound = k < bound ? k : bound;
-                }
-                for (int i = tid; i < C * a.n_top; i += LP_NT)
-                    if (lists[i] >= bound && lists[i]) s_all[atomicAdd(&s_cnt[0], 1)] = lists[i];
-                __syncthreads();
-                lp_rank(s_all, s_cnt[0], s_best, a.n_top, tid);
-            }
-        }
-        cl.sync();  // the other CTAs' shared memory stays until it has been read
+        if (tid == 0) *cl.map_shared_rank(&s_stats[rank], 0) = s_cta;
+        if constexpr (TOP)
+            if (tid < a.n_top) cl.map_shared_rank(s_lists, 0)[rank * a.n_top + tid] = s_best[tid];
+        cluster_arrive();
         if (rank != 0) return;
-        if (tid == 0) s_cta = s_stat[0];
+        cluster_wait();
+        if (warp == 0) {
+            LpStat t = s_stats[lane % C];
+            lp_join_lanes(t, C);
+            if (lane == 0) s_cta = t;
+        }
+        if constexpr (TOP) {
+            // ceil(n / C) values of every CTA reach the least of the CTAs' ceil(n / C)-th ones, n
+            // values at least: only what reaches it is ranked
+            const int deep = (a.n_top + C - 1) / C;
+            if (tid == 0) s_cnt[0] = 0;
+            __syncthreads();
+            uint64_t bound = lane < C ? s_lists[lane * a.n_top + deep - 1] : ~0ull;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                const uint64_t other = __shfl_xor_sync(0xffffffffu, bound, o);
+                bound = other < bound ? other : bound;
+            }
+            for (int i = tid; i < C * a.n_top; i += LP_NT)
+                if (s_lists[i] >= bound && s_lists[i]) s_all[atomicAdd(&s_cnt[0], 1)] = s_lists[i];
+            __syncthreads();
+            lp_rank(s_all, s_cnt[0], s_best, a.n_top, tid);
+        }
     }
     __syncthreads();
     const LpStat t = s_cta;
@@ -482,9 +485,9 @@ int token_logprobs(pi_ctx* ctx, const void* logits, int32_t dtype, int64_t T, in
     if ((uintptr_t)logits % es) return pi_set_error(ctx, PI_ERR_ARG, "logprobs: logits are not aligned to their type");
     PiDeviceGuard dev(ctx->device);
     LogprobArgs a{logits, T, V, ld, targets, n_targets, n_top, 1, logp, entropy, top_ids, top_logp, ctx->dev_err};
-    // CTAs of a row: while four per SM are not reached and each has two loads a thread left
+    // CTAs of a row: as long as all of the grid's run at once and each has two loads a thread
     const int64_t nvec = V * es / 16, sms = ctx->sm_count > 0 ? ctx->sm_count : 148;
-    while (a.C < LP_MAXC && T * a.C * 2 <= 4 * sms && nvec >= (int64_t)a.C * 2 * 2 * LP_NT) a.C *= 2;
+    while (a.C < LP_MAXC && T * a.C * 2 <= LP_OCC * sms && nvec >= (int64_t)a.C * 2 * 2 * LP_NT) a.C *= 2;
     PiProfScope ps(ctx, st, "k_token_logprobs");
     const cudaError_t e = dtype == PI_QT_F32   ? launch_logprobs<float>(ctx, a, st)
                           : dtype == PI_QT_F16 ? launch_logprobs<__half>(ctx, a, st)

@@ -19,6 +19,7 @@
 
 #include <algorithm>
 #include <exception>
+#include <map>
 
 namespace cg = cooperative_groups;
 
@@ -29,6 +30,13 @@ struct pi_proj {
     int64_t units = 0;   // pairs of 32-element blocks of a row, the last padded with zeros
     int64_t tiles = 0;   // tiles of 16 rows, the last padded with zero rows
     uint8_t* w = nullptr;
+    // how k_proj_gemm is launched for a number of n-tiles, found at its first use
+    struct Plan {
+        int ks, cu, nchunk, sums;
+        size_t smem;
+    };
+    mutable std::mutex mu;
+    mutable std::map<int64_t, Plan> plans;
 };
 
 namespace {
@@ -139,7 +147,8 @@ PI_DEV void ld_adapter8(const void* base, int64_t off, int dtype, float* f) {
 // so that a run of units of one chunk is one contiguous piece. Lane 4 g + i holds token g of
 // the n-tile:
 //   Q8_0: 512 B, the lane's {k 4i.., k 16+4i..} of either block, then 64 B of scales, i's
-//         {tokens 2i, 2i+1} of either block
+//         {tokens 2i, 2i+1} of either block (f32: as f16 the conversions cost more, 150 us
+//         against 137 at n_out 151936 and 64 tokens, than the reads saved)
 //   Q4_0: per block and k-step (k 8i + 4 step ..) 512 B, the lane's {hi, hi, lo, lo}
 // ---------------------------------------------------------------------------
 template <int QT>
@@ -273,7 +282,7 @@ __global__ __launch_bounds__(PREP_T) void k_proj_prep(const float* __restrict__ 
         float acc[PREP_R] = {};
         const float* xr = x + t * n_in;
         const int64_t base = ((int64_t)a * L.R + r0) * n_in;
-#pragma unroll 2
+#pragma unroll 4
         for (int64_t k = part * 256 + lane * 8; k < n_in; k += 256 * PREP_S) {
             const float4 u = *reinterpret_cast<const float4*>(xr + k);
             const float4 v = *reinterpret_cast<const float4*>(xr + k + 4);
@@ -324,6 +333,7 @@ struct ProjArgs {
     int ks;      // CTAs that share the blocks of their rows
     int cu;      // units of a part that are staged together
     int nchunk;  // such pieces of a part
+    int sums;    // where the parts' sums lie in shared memory
 };
 
 PI_DEV void mma_s8(int (&c)[4], const uint4& a, const uint2& b) {
@@ -372,6 +382,7 @@ PI_DEV void cp_async16(uint32_t dst, const void* src) {
 
 constexpr int GEMM_T = 256;
 constexpr int GEMM_W = GEMM_T / 32;
+constexpr size_t GEMM_SMEM = 200 * 1024;
 constexpr int RING = 4;  // units a warp holds or has in flight (4 KB of Q8_0 weights)
 
 // CTA = 8 warps of 16 rows each; blockIdx.x = the CTA's part of the blocks (the ks CTAs of a
@@ -398,6 +409,7 @@ __global__ __launch_bounds__(GEMM_T, 2) void k_proj_gemm(const ProjArgs p) {
     const int ncol = (int)min((int64_t)NC, p.T - t0);
     const int ub = (int)(p.units * part / ks), ue = (int)(p.units * (part + 1) / ks);
     const bool live = tile < p.tiles;
+    if (ks > 1) cluster_arrive();  // the others write into this CTA's shared memory when they know that it runs
     const uint8_t* wt = p.w + tile * p.units * UB;
     UnitRegs<QT> ring[D];
     if (live) {
@@ -535,22 +547,25 @@ __global__ __launch_bounds__(GEMM_T, 2) void k_proj_gemm(const ProjArgs p) {
         acc[n][2] = v.x;
         acc[n][3] = v.y;
     }
-    if (ks > 1) {  // n-tile n belongs to CTA n % ks of the cluster from here on
+    if (ks > 1) {  // n-tile n belongs to CTA n % ks of the cluster from here on: the parts go there
         cg::cluster_group cl = cg::this_cluster();
-        float* sums = reinterpret_cast<float*>(s_x);
-        __syncthreads();
+        float4* sums = reinterpret_cast<float4*>(s_x + p.sums) + warp * 32 + lane;  // [n / ks][part][warp][lane]
+        cluster_wait();
+        if (live) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-            *reinterpret_cast<float4*>(sums + ((warp * NT + n) * 32 + lane) * 4) =
-                make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
-        cl.sync();
+            for (int n = 0; n < NT; ++n)
+                cl.map_shared_rank(sums, n % ks)[((n / ks) * ks + part) * GEMM_T] =
+                    make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
+        }
+        cluster_arrive();
+        if (part >= NT) return;  // no n-tile is this CTA's
+        cluster_wait();
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             if (n % ks != part) continue;
             float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
             for (int q = 0; q < ks; ++q) {
-                const float4 v = *reinterpret_cast<const float4*>(cl.map_shared_rank(sums, q) +
-                                                                  ((warp * NT + n) * 32 + lane) * 4);
+                const float4 v = sums[((n / ks) * ks + q) * GEMM_T];
                 t.x += v.x;
                 t.y += v.y;
                 t.z += v.z;
@@ -561,7 +576,6 @@ __global__ __launch_bounds__(GEMM_T, 2) void k_proj_gemm(const ProjArgs p) {
             acc[n][2] = t.z;
             acc[n][3] = t.w;
         }
-        cl.sync();  // the other CTAs' shared memory stays until it has been read
     }
     if (!live) return;
     if (QT == PI_QT_Q4_0) {
@@ -793,36 +807,74 @@ int proj_create(pi_ctx* ctx, const void* raw, uint64_t raw_len, int32_t qtype, i
     return PI_OK;
 }
 
+// Parts of the blocks (ks) and stages. The time of a grid is about the rounds of CTAs that run at
+// once times the units of a part plus what a CTA costs beside them (start, stage and join,
+// about a dozen units' time). How many clusters run at once the runtime knows: clusters of
+// three or five leave SMs of a GPC empty.
 template <int QT, int NT>
-cudaError_t launch_gemm(ProjArgs a, int64_t sms, cudaStream_t st) {
-    constexpr int XU = NT * xunit_bytes<QT>(), D = RING;
-    const int64_t sets = (a.tiles + GEMM_W - 1) / GEMM_W, chunks = (a.T + 8 * NT - 1) / (8 * NT);
-    // Parts of the blocks: the time is about the rounds of CTAs, two to an SM, times the units
-    // of a part plus what a CTA costs beside them (start, stage and join, about a dozen units)
-    a.ks = 1;
-    int64_t best = INT64_MAX;
-    for (int ks = 1; ks <= 8 && ks <= a.units; ++ks) {
-        const int64_t rounds = (sets * chunks * ks + 2 * sms - 1) / (2 * sms);
-        const int64_t cost = rounds * ((a.units + ks - 1) / ks + 12);
-        if (cost < best) {
-            best = cost;
-            a.ks = ks;
+pi_proj::Plan plan_gemm(const pi_proj* P, int64_t T, int64_t sms) {
+    constexpr int XU = NT * xunit_bytes<QT>();
+    const int64_t sets = (P->tiles + GEMM_W - 1) / GEMM_W, chunks = (T + 8 * NT - 1) / (8 * NT);
+    auto kern = k_proj_gemm<QT, NT>;
+    pi_smem_attr((const void*)kern, GEMM_SMEM);
+    pi_proj::Plan best = {};
+    int64_t least = INT64_MAX;
+    for (int ks = 1; ks <= 8 && ks <= P->units; ++ks) {
+        pi_proj::Plan q;
+        q.ks = ks;
+        // a part is staged whole where two CTAs of an SM have room for it beside the sums, in
+        // pieces of a multiple of RING units otherwise
+        const int64_t sums = ks > 1 ? (int64_t)((NT + ks - 1) / ks) * ks * GEMM_T * 16 : 0;
+        const int64_t budget = 108 * 1024 - sums, part = (P->units + ks - 1) / ks;
+        q.cu = (int)part;
+        if (part * XU > budget) q.cu = (int)std::max<int64_t>(RING, budget / 2 / XU / RING * RING);
+        q.nchunk = (int)((part + q.cu - 1) / q.cu);
+        q.sums = std::min(q.nchunk, 2) * q.cu * XU;
+        q.smem = (size_t)(q.sums + sums);
+        if (q.smem > GEMM_SMEM) continue;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(sets * ks), (unsigned)chunks);
+        cfg.blockDim = dim3(GEMM_T);
+        cfg.dynamicSmemBytes = q.smem;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = (unsigned)ks;
+        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        int clusters = 0;
+        if (cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg) != cudaSuccess || clusters < 1) {
+            cudaGetLastError();
+            clusters = (int)(sms / ks);
+        }
+        const int64_t rounds = (sets * chunks + clusters - 1) / clusters, cost = rounds * (part + 12);
+        if (cost < least) {
+            least = cost;
+            best = q;
         }
     }
-    // A part is staged whole where two CTAs of an SM have room for it, in pieces of a multiple
-    // of D units otherwise
-    const int64_t budget = 100 * 1024, part = (a.units + a.ks - 1) / a.ks;
-    a.cu = (int)part;
-    if (part * XU > budget) a.cu = (int)std::max<int64_t>(D, budget / 2 / XU / D * D);
-    a.nchunk = (int)((part + a.cu - 1) / a.cu);
-    const size_t sums = a.ks > 1 ? (size_t)GEMM_W * NT * 512 : 0;
-    const size_t smem = std::max<size_t>((size_t)std::min(a.nchunk, 2) * a.cu * XU, sums);
-    auto kern = k_proj_gemm<QT, NT>;
-    pi_smem_attr((const void*)kern, smem);
+    return best;
+}
+
+template <int QT, int NT>
+cudaError_t launch_gemm(const pi_proj* P, ProjArgs a, int64_t sms, cudaStream_t st) {
+    pi_proj::Plan q;
+    {
+        std::lock_guard<std::mutex> g(P->mu);
+        const int64_t key = (a.T + 7) / 8;  // the plan goes by n-tiles
+        auto it = P->plans.find(key);
+        if (it == P->plans.end()) it = P->plans.emplace(key, plan_gemm<QT, NT>(P, a.T, sms)).first;
+        q = it->second;
+    }
+    a.ks = q.ks;
+    a.cu = q.cu;
+    a.nchunk = q.nchunk;
+    a.sums = q.sums;
+    const int64_t sets = (a.tiles + GEMM_W - 1) / GEMM_W, chunks = (a.T + 8 * NT - 1) / (8 * NT);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(sets * a.ks), (unsigned)chunks);
     cfg.blockDim = dim3(GEMM_T);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = q.smem;
     cfg.stream = st;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -832,20 +884,20 @@ cudaError_t launch_gemm(ProjArgs a, int64_t sms, cudaStream_t st) {
     at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = a.ks > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kern, a);
+    return cudaLaunchKernelEx(&cfg, k_proj_gemm<QT, NT>, a);
 }
 
 template <int QT>
-cudaError_t dispatch_gemm(const ProjArgs& a, int NT, int64_t sms, cudaStream_t st) {
+cudaError_t dispatch_gemm(const pi_proj* P, const ProjArgs& a, int NT, int64_t sms, cudaStream_t st) {
     switch (NT) {
-        case 1: return launch_gemm<QT, 1>(a, sms, st);
-        case 2: return launch_gemm<QT, 2>(a, sms, st);
-        case 3: return launch_gemm<QT, 3>(a, sms, st);
-        case 4: return launch_gemm<QT, 4>(a, sms, st);
-        case 5: return launch_gemm<QT, 5>(a, sms, st);
-        case 6: return launch_gemm<QT, 6>(a, sms, st);
-        case 7: return launch_gemm<QT, 7>(a, sms, st);
-        default: return launch_gemm<QT, 8>(a, sms, st);
+        case 1: return launch_gemm<QT, 1>(P, a, sms, st);
+        case 2: return launch_gemm<QT, 2>(P, a, sms, st);
+        case 3: return launch_gemm<QT, 3>(P, a, sms, st);
+        case 4: return launch_gemm<QT, 4>(P, a, sms, st);
+        case 5: return launch_gemm<QT, 5>(P, a, sms, st);
+        case 6: return launch_gemm<QT, 6>(P, a, sms, st);
+        case 7: return launch_gemm<QT, 7>(P, a, sms, st);
+        default: return launch_gemm<QT, 8>(P, a, sms, st);
     }
 }
 
@@ -894,9 +946,9 @@ int proj_forward(pi_ctx* ctx, const pi_proj* P, const float* x, int64_t T, const
     }
     {
         PiProfScope ps(ctx, st, "k_proj_gemm");
-        const ProjArgs a{P->w, B.xf, B.xs, B.h, y, L, T, P->n_out, P->units, P->tiles, 1, 1, 1};
+        const ProjArgs a{P->w, B.xf, B.xs, B.h, y, L, T, P->n_out, P->units, P->tiles, 1, 1, 1, 0};
         const int64_t sms = ctx->sm_count > 0 ? ctx->sm_count : 148;
-        const cudaError_t e = q8 ? dispatch_gemm<PI_QT_Q8_0>(a, NT, sms, st) : dispatch_gemm<PI_QT_Q4_0>(a, NT, sms, st);
+        const cudaError_t e = q8 ? dispatch_gemm<PI_QT_Q8_0>(P, a, NT, sms, st) : dispatch_gemm<PI_QT_Q4_0>(P, a, NT, sms, st);
         if (e != cudaSuccess) return pi_cuda_check(ctx, e, "projection");
     }
     return pi_cuda_check(ctx, cudaGetLastError(), "projection") ? PI_ERR_CUDA : PI_OK;
