@@ -26,10 +26,14 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int LP_NT = 256;       // threads of a CTA
-constexpr int LP_W = LP_NT / 32;
-constexpr int LP_U = 2;          // 16-byte loads of a step; the next step's are in flight
-constexpr int LP_OCC = 4;        // CTAs of an SM
+constexpr int LP_U = 4;          // 16-byte loads of a step
+// NT threads work on a row together: 256, or one warp where there are rows for all SMs. What does
+// not shrink with the row (threshold, joins, ranking) is then paid by one warp instead of
+// eight: 2048 rows of 32000 bf16 take 38 us, with 256 threads a row 41.
+template <int NT>
+constexpr int lp_occ() { return NT == 256 ? 3 : 16; }  // CTAs of an SM
+template <int NT>
+constexpr int lp_ring() { return NT == 256 ? 8 : 12; }  // 16-byte loads a thread has in flight or at hand
 constexpr int LP_MAXC = 16;      // CTAs of a cluster at most
 constexpr int LP_MAXTOP = 32;    // alternatives at most
 constexpr float LP_LOG2E = 1.4426950408889634f;
@@ -61,15 +65,6 @@ PI_DEV float ex2(float a) {
 // the type's lowest) adds 0 to both sums instead of 0 * inf; NaN stays NaN.
 PI_DEV float lp_shift(float x, float m) { return max_nan(x - m, -200.0f); }
 
-PI_DEV void lp_join(LpStat& a, const LpStat& b) {
-    const float m = fmaxf(a.m, b.m);
-    const float da = lp_shift(a.m, m), db = lp_shift(b.m, m);
-    const float ea = ex2(da * LP_LOG2E), eb = ex2(db * LP_LOG2E);
-    a.w = fmaf(da, a.s, a.w) * ea + fmaf(db, b.s, b.w) * eb;
-    a.s = a.s * ea + b.s * eb;
-    a.m = m;
-}
-
 template <int N>
 PI_DEV float lp_max(const float* f) {
     float a = fmaxf(f[0], f[1]), b = fmaxf(f[2], f[3]);
@@ -80,6 +75,12 @@ PI_DEV float lp_max(const float* f) {
     return fmaxf(a, b);
 }
 
+// Largest of the warp's values, NaN dropped.
+PI_DEV float warp_max(float v) {
+    float r;
+    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
 // One 64-bit key per value: larger for a larger logit and, where they tie (-0 and 0 too),
 // for a lower index. 0 stands for no value; values above -inf have keys above 0.
 PI_DEV uint64_t lp_key(float v, uint32_t i) {
@@ -137,7 +138,11 @@ struct LpTop {
 
     // keeps the n best of the buffer, in order
     PI_DEV void compact() {
-        constexpr int P = CAP / 32;
+        if (cnt <= 64) keep_best<2>();
+        else keep_best<CAP / 32>();
+    }
+    template <int P>  // P keys a lane
+    PI_DEV void keep_best() {
         uint64_t k[P];
 #pragma unroll
         for (int i = 0; i < P; ++i) k[i] = lane + 32 * i < cnt ? buf[lane + 32 * i] : 0;
@@ -174,14 +179,23 @@ struct LpTop {
             cnt += __popc(b);
         }
         __syncwarp();
+        // A threshold that stays behind lets value after value in (32000 values, n = 1, threshold of
+        // the first 512: 62 of them, one in most steps): it follows.
+        if (n == 1) {
+            thr = fmaxf(thr, warp_max(vmax));
+            incl = false;
+        } else if (cnt >= n + 24) {
+            compact();
+        }
     }
 };
 
 // The n best of `cnt` distinct keys in `all` to best[0..n) (0 where there are fewer): a
 // key's place is the number of larger ones, counted by four lanes.
+template <int NT>
 PI_DEV void lp_rank(const uint64_t* all, int cnt, uint64_t* best, int n, int tid) {
     if (tid < n && tid >= cnt) best[tid] = 0;
-    for (int i0 = 0; i0 < cnt; i0 += LP_NT / 4) {
+    for (int i0 = 0; i0 < cnt; i0 += NT / 4) {
         const int i = i0 + (tid >> 2);
         const uint64_t k = i < cnt ? all[i] : ~0ull;
         int r = 0;
@@ -192,59 +206,95 @@ PI_DEV void lp_rank(const uint64_t* all, int cnt, uint64_t* best, int n, int tid
     }
 }
 
-// Joins the states of the lanes whose numbers differ below `width`, a power of two.
-PI_DEV void lp_join_lanes(LpStat& st, int width) {
-    for (int o = width >> 1; o > 0; o >>= 1) {
-        LpStat b;
-        b.m = __shfl_xor_sync(0xffffffffu, st.m, o);
-        b.s = __shfl_xor_sync(0xffffffffu, st.s, o);
-        b.w = __shfl_xor_sync(0xffffffffu, st.w, o);
-        lp_join(st, b);
-    }
+// The joined state of a warp's lanes (in every lane): the common maximum first, one rescaling,
+// then plain sums.
+PI_DEV void lp_join_warp(LpStat& st) {
+    const float m = warp_max(st.m), dm = lp_shift(st.m, m), e = ex2(dm * LP_LOG2E);
+    st.w = warp_sum(fmaf(dm, st.s, st.w) * e);
+    st.s = warp_sum(st.s * e);
+    st.m = m;
 }
 
-// Row blockIdx.x / C, share blockIdx.x % C. The first LP_U loads of a thread give, over
-// groups of four lanes, 64 maxima: the n-th largest of them is reached by n values at
-// least, so only what reaches it is kept from the start (about n values of the first
-// 2048 or 4096, then n / i of the i-th step), and the buffers hardly ever fill.
-template <typename ET, bool TOP>
-__global__ __launch_bounds__(LP_NT, LP_OCC) void k_token_logprobs(const LogprobArgs a) {
+// Row blockIdx.x / C, share blockIdx.x % C. The first LP_U loads of a thread give maxima of
+// groups: the n-th largest of the warps' (n <= 8) or of 64 groups of four lanes (a warp alone:
+// of its lanes) is reached by n values at least, so only what reaches it is kept from the start
+// (with 256 threads about n values of the first 4096 or 8192, then n / i of the i-th step), and
+// the buffers hardly ever fill.
+template <typename ET, bool TOP, int NT>
+__global__ __launch_bounds__(NT, lp_occ<NT>()) void k_token_logprobs(const LogprobArgs a) {
+    constexpr int LP_NT = NT, LP_W = NT / 32, LP_D = lp_ring<NT>();
+    constexpr int GROUP = NT == 256 ? 4 : 1, GROUPS = NT / GROUP;  // groups of lanes whose maxima give the threshold
+    constexpr int KEYS = NT == 256 ? LP_MAXC * LP_MAXTOP : 320;    // keys ranked together; one warp has no cluster
     constexpr int NV = 16 / (int)sizeof(ET);
     constexpr int CAP = 64 + 32 * NV;  // n kept after compact() and one load of every lane
     __shared__ uint64_t s_buf[TOP ? LP_W * CAP : 1];
-    __shared__ uint64_t s_all[TOP ? LP_MAXC * LP_MAXTOP : 1];
-    __shared__ uint64_t s_lists[TOP ? LP_MAXC * LP_MAXTOP : 1];  // the cluster's lists, in its first CTA
-    __shared__ LpStat s_stats[LP_MAXC];                          // and its states
+    __shared__ uint64_t s_all[TOP ? KEYS : 1];
+    __shared__ uint64_t s_lists[TOP && NT == 256 ? LP_MAXC * LP_MAXTOP : 1];  // the cluster's lists, in its first CTA
+    __shared__ LpStat s_stats[LP_MAXC];                                       // and its states
     __shared__ uint64_t s_best[LP_MAXTOP];
     __shared__ LpStat s_stat[LP_W], s_cta;
-    __shared__ float s_max[64], s_thr;
+    __shared__ float s_max[GROUPS], s_thr;
     __shared__ int s_cnt[LP_W];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int C = a.C;
-    const int64_t row = blockIdx.x / C;
-    const int rank = (int)(blockIdx.x - row * C);
+    const int C = NT == 256 ? a.C : 1;
+    const int row32 = (int)(blockIdx.x / (unsigned)C), rank = (int)blockIdx.x - row32 * C;
+    const int64_t row = row32;
     const ET* x = reinterpret_cast<const ET*>(a.logits) + row * a.ld;
     // values before the first 16-byte boundary and after the last whole 16 bytes are read
     // one by one by the first warp of the row
-    const int64_t head = min((int64_t)(((16 - ((uintptr_t)x & 15)) & 15) / sizeof(ET)), a.V);
-    const int64_t nvec = (a.V - head) / NV, tail = head + nvec * NV;
+    const int head = (int)min((int64_t)(((16 - ((uintptr_t)x & 15)) & 15) / sizeof(ET)), a.V);
+    const int nvec = (int)((a.V - head) / NV), tail = head + nvec * NV;
     const int4* xv = reinterpret_cast<const int4*>(x + head);
-    const int64_t step = (int64_t)C * LP_NT;
+    const int step = C * LP_NT;
+    // the row's results from its joined state and s_best, by `nthr` threads
+    auto answer = [&](const LpStat& t, int i0, int nthr) {
+        // s == 0: the row's mask leaves nothing; s NaN: a NaN or +inf, no distribution
+        const bool none = t.s == 0.0f, bad = t.s != t.s;
+        const float log_s = none ? 0.0f : logf(t.s), nan = __int_as_float(0x7fffffff);
+        if (i0 == 0 && a.entropy) a.entropy[row] = none ? 0.0f : (bad ? nan : log_s - t.w / t.s);
+        for (int64_t j = i0; j < a.n_targets; j += nthr) {
+            const int64_t v = a.targets[row * a.n_targets + j];
+            float r = 0.0f;  // a negative target is no token
+            if (v >= a.V) {
+                atomicOr(a.err, PI_DEVERR_INDEX);
+                r = nan;
+            } else if (v >= 0) {
+                const float xt = lp_float(x[v]);
+                r = none ? -INFINITY : (bad ? nan : (xt - t.m) - log_s);
+            }
+            a.logp[row * a.n_targets + j] = r;
+        }
+        if constexpr (TOP) {
+            if (i0 < a.n_top) {
+                const uint64_t k = bad ? 0 : s_best[i0];
+                a.top_ids[row * a.n_top + i0] = k ? (int32_t)lp_key_index(k) : -1;
+                a.top_logp[row * a.n_top + i0] = bad ? nan : (k ? (lp_key_value(k) - t.m) - log_s : -INFINITY);
+            }
+        }
+    };
     const bool edges = rank == 0 && warp == 0;
     // the first CTA of the cluster must run before the others write into its shared memory
-    if (C > 1) cluster_arrive();
+    if (NT == 256 && C > 1) cluster_arrive();
 
-    LpStat st{LP_LOWEST, 0.0f, 0.0f};
-    auto scalar = [&](float v) {
-        if (v > st.m) {
-            const float dm = lp_shift(st.m, v), e = ex2(dm * LP_LOG2E);
-            st.w = fmaf(dm, st.s, st.w) * e;
-            st.s *= e;
-            st.m = v;
-        }
-        const float t = lp_shift(v, st.m), e = ex2(t * LP_LOG2E);
-        st.s += e;
-        st.w = fmaf(t, e, st.w);
+    // this thread's maximum and packed sums of e^(x - m) and (x - m) e^(x - m)
+    float m = LP_LOWEST;
+    uint64_t s2 = 0, w2 = 0;
+    auto raise = [&](float to) {
+        const float dm = lp_shift(m, to), e = ex2(dm * LP_LOG2E);
+        const uint64_t e2 = pack2(e, e);
+        w2 = mul2(fma2(pack2(dm, dm), s2, w2), e2);
+        s2 = mul2(s2, e2);
+        m = to;
+    };
+    auto pair = [&](float x0, float x1) {
+        float2 t = unpack2(add2(pack2(x0, x1), pack2(-m, -m)));
+        t.x = max_nan(t.x, -200.0f);
+        t.y = max_nan(t.y, -200.0f);
+        const uint64_t tt = pack2(t.x, t.y);
+        const float2 g = unpack2(mul2(tt, pack2(LP_LOG2E, LP_LOG2E)));
+        const uint64_t e = pack2(ex2(g.x), ex2(g.y));
+        s2 = add2(s2, e);
+        w2 = fma2(tt, e, w2);
     };
     LpTop<CAP> top;
     if constexpr (TOP) {
@@ -254,132 +304,162 @@ __global__ __launch_bounds__(LP_NT, LP_OCC) void k_token_logprobs(const LogprobA
     }
     if (edges) {
         const float v = lane < head ? lp_float(x[lane]) : -INFINITY;
-        if (lane < head) scalar(v);
+        if (lane < head) {
+            if (v > m) raise(v);
+            pair(v, -INFINITY);
+        }
         if constexpr (TOP) top.template add<1>(&v, v, (uint32_t)lane);
     }
-    // the next LP_U loads are on their way while the current ones are worked on
-    int4 q[LP_U], qn[LP_U];
-    int64_t v0 = (int64_t)rank * LP_NT + tid;
+    // Loads go through a ring in shared memory, of which a thread reads only what it copied itself
+    // (no barrier): 32 KB a CTA in flight. In registers 8 KB were (2048 rows of 32000 bf16: 47
+    // us, 2.8 TB/s).
+    const int minus_inf = sizeof(ET) == 4 ? (int)0xff800000 : (std::is_same_v<ET, __half> ? (int)0xfc00fc00 : (int)0xff80ff80);
+    const int4 none = make_int4(minus_inf, minus_inf, minus_inf, minus_inf);
+    extern __shared__ __align__(16) int4 s_ring[];
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(s_ring + tid);
+    int v0 = rank * LP_NT + tid, slot = 0;
+    auto request = [&](int v, int at) {  // a step's loads, one group
 #pragma unroll
-    for (int u = 0; u < LP_U; ++u)
-        if (v0 + u * step < nvec) qn[u] = ld_stream(xv + v0 + u * step);
+        for (int u = 0; u < LP_U; ++u)
+            if (v + u * step < nvec)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ring + (at + u) * LP_NT * 16),
+                             "l"(xv + v + u * step)
+                             : "memory");
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < LP_D; i += LP_U) request(v0 + i * step, i);
     bool first = true;
     for (; v0 - tid < nvec || first; v0 += LP_U * step) {
+        float f[LP_U][NV], vmax[LP_U], mx = -INFINITY;
+        asm volatile("cp.async.wait_group %0;" ::"n"(LP_D / LP_U - 1) : "memory");
 #pragma unroll
         for (int u = 0; u < LP_U; ++u) {
-            q[u] = qn[u];
-            if (v0 + (LP_U + u) * step < nvec) qn[u] = ld_stream(xv + v0 + (LP_U + u) * step);
+            lp_unpack<ET>(v0 + u * step < nvec ? s_ring[(slot + u) * LP_NT + tid] : none, f[u]);  // behind the end: -inf
+            vmax[u] = lp_max<NV>(f[u]);
+            mx = fmaxf(mx, vmax[u]);
         }
+        request(v0 + LP_D * step, slot);
+        slot = slot + LP_U == LP_D ? 0 : slot + LP_U;
         if constexpr (TOP) {
             if (first) {
-                float mx = -INFINITY;
+                if (a.n_top <= LP_W) {
+                    const float w = warp_max(mx);
+                    if (lane == 0) s_max[warp] = w;
+                    __syncthreads();
+                    const float mine = s_max[lane % LP_W];
+                    int r = 0;
 #pragma unroll
-                for (int u = 0; u < LP_U; ++u)
-                    if (v0 + u * step < nvec) {
-                        float f[NV];
-                        lp_unpack<ET>(q[u], f);
-                        mx = fmaxf(mx, lp_max<NV>(f));
-                    }
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                if ((lane & 3) == 0) s_max[tid >> 2] = mx;
-                __syncthreads();
-                {
-                    const int i = tid >> 2;  // four lanes count the maxima above the i-th
+                    for (int o = 0; o < LP_W; ++o) r += s_max[o] > mine || (s_max[o] == mine && o < lane % LP_W);
+                    const uint32_t b = __ballot_sync(0xffffffffu, r == a.n_top - 1);
+                    top.thr = __shfl_sync(0xffffffffu, mine, __ffs(b) - 1);
+                } else {
+                    float w = mx;
+#pragma unroll
+                    for (int o = 1; o < GROUP; o <<= 1) w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, o));
+                    if (tid % GROUP == 0) s_max[tid / GROUP] = w;
+                    __syncthreads();
+                    const int i = tid / GROUP;  // the lanes of a group count the maxima above theirs
                     const float mine = s_max[i];
                     int r = 0;
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const int o = (tid & 3) + 4 * j;
+                    for (int j = 0; j < GROUPS / GROUP; ++j) {
+                        const int o = tid % GROUP + GROUP * j;
                         r += s_max[o] > mine || (s_max[o] == mine && o < i);
                     }
-                    r += __shfl_xor_sync(0xffffffffu, r, 1);
-                    r += __shfl_xor_sync(0xffffffffu, r, 2);
+#pragma unroll
+                    for (int o = 1; o < GROUP; o <<= 1) r += __shfl_xor_sync(0xffffffffu, r, o);
                     if (r == a.n_top - 1) s_thr = mine;
+                    __syncthreads();
+                    top.thr = s_thr;
                 }
-                __syncthreads();
-                top.thr = s_thr;
-                top.incl = s_thr > -INFINITY;
+                top.incl = top.thr > -INFINITY;
             }
         }
+        if (mx > m) raise(mx);
 #pragma unroll
-        for (int u = 0; u < LP_U; ++u) {
-            const bool live = v0 + u * step < nvec;
-            float f[NV];
-            float vmax = -INFINITY;
-            if (live) {
-                lp_unpack<ET>(q[u], f);
-                vmax = lp_max<NV>(f);
-                if (vmax > st.m) {
-                    const float dm = lp_shift(st.m, vmax), e = ex2(dm * LP_LOG2E);
-                    st.w = fmaf(dm, st.s, st.w) * e;
-                    st.s *= e;
-                    st.m = vmax;
-                }
-                const uint64_t m2 = pack2(-st.m, -st.m), l2 = pack2(LP_LOG2E, LP_LOG2E);
-                uint64_t s2 = 0, w2 = 0;
+        for (int u = 0; u < LP_U; ++u)
 #pragma unroll
-                for (int j = 0; j < NV; j += 2) {
-                    float2 t = unpack2(add2(pack2(f[j], f[j + 1]), m2));
-                    t.x = max_nan(t.x, -200.0f);
-                    t.y = max_nan(t.y, -200.0f);
-                    const uint64_t tt = pack2(t.x, t.y);
-                    const float2 g = unpack2(mul2(tt, l2));
-                    const uint64_t e = pack2(ex2(g.x), ex2(g.y));
-                    s2 = add2(s2, e);
-                    w2 = fma2(tt, e, w2);
-                }
-                const float2 sp = unpack2(s2), wp = unpack2(w2);
-                st.s += sp.x + sp.y;
-                st.w += wp.x + wp.y;
-            } else {
+            for (int j = 0; j < NV; j += 2) pair(f[u][j], f[u][j + 1]);
+        if constexpr (TOP) {
+            if (__any_sync(0xffffffffu, top.passes(mx)))
 #pragma unroll
-                for (int j = 0; j < NV; ++j) f[j] = -INFINITY;
-            }
-            if constexpr (TOP) top.template add<NV>(f, vmax, (uint32_t)(head + (v0 + u * step) * NV));
+                for (int u = 0; u < LP_U; ++u)
+                    top.template add<NV>(f[u], vmax[u], (uint32_t)(head + (v0 + u * step) * NV));
+            top.incl = false;
         }
-        if constexpr (TOP) top.incl = false;
         first = false;
     }
     if (edges) {
-        const int64_t i = tail + lane;
+        const int i = tail + lane;
         const float v = i < a.V ? lp_float(x[i]) : -INFINITY;
-        if (i < a.V) scalar(v);
+        if (i < a.V) {
+            if (v > m) raise(v);
+            pair(v, -INFINITY);
+        }
         if constexpr (TOP) top.template add<1>(&v, v, (uint32_t)i);
     }
 
+    const float2 ss = unpack2(s2), ww = unpack2(w2);
+    LpStat st{m, ss.x + ss.y, ww.x + ww.y};
     // join: lanes, warps, then the CTAs of the cluster
-    lp_join_lanes(st, 32);
+    lp_join_warp(st);
     if (lane == 0) s_stat[warp] = st;
     if constexpr (TOP) {
         if (lane == 0) s_cnt[warp] = top.cnt;
         __syncthreads();
-        int total = 0;
-        for (int i = 0; i < LP_W; ++i) total += s_cnt[i];
-        if (total > LP_NT) {
-            __syncthreads();
-            if (top.cnt > a.n_top) top.compact();
-            if (lane == 0) s_cnt[warp] = top.cnt;
-            __syncthreads();
-        }
-        int at = 0;
-        total = 0;
+        int at = 0, total = 0;
         for (int i = 0; i < LP_W; ++i) {
             if (i < warp) at += s_cnt[i];
             total += s_cnt[i];
         }
+        if (NT == 256 && total > NT) {
+            __syncthreads();
+            if (top.cnt > a.n_top) top.compact();
+            if (lane == 0) s_cnt[warp] = top.cnt;
+            __syncthreads();
+            at = total = 0;
+            for (int i = 0; i < LP_W; ++i) {
+                if (i < warp) at += s_cnt[i];
+                total += s_cnt[i];
+            }
+        }
         for (int i = lane; i < top.cnt; i += 32) s_all[at + i] = top.buf[i];
         __syncthreads();
-        lp_rank(s_all, total, s_best, a.n_top, tid);
+        if ((NT == 32 || C == 1) && total <= 32) {  // few keys: the first warp ranks them, the others are done
+            if (warp != 0) return;
+            const uint64_t k = lane < total ? s_all[lane] : 0;
+            int r = 0;
+            for (int j = 0; j < total; ++j) r += s_all[j] > k;
+            if (lane < a.n_top) s_best[lane] = 0;
+            __syncwarp();
+            if (lane < total && r < a.n_top) s_best[r] = k;
+            __syncwarp();
+            LpStat t = s_stat[lane % LP_W];
+            if (lane >= LP_W) t.s = t.w = 0.0f;
+            lp_join_warp(t);
+            answer(t, lane, 32);
+            return;
+        }
+        lp_rank<NT>(s_all, total, s_best, a.n_top, tid);
     } else {
         __syncthreads();
+        if (C == 1) {
+            if (warp != 0) return;
+            LpStat t = s_stat[lane % LP_W];
+            if (lane >= LP_W) t.s = t.w = 0.0f;
+            lp_join_warp(t);
+            answer(t, lane, 32);
+            return;
+        }
     }
     if (warp == 0) {
         LpStat t = s_stat[lane % LP_W];
-        lp_join_lanes(t, LP_W);
+        if (lane >= LP_W) t.s = t.w = 0.0f;
+        lp_join_warp(t);
         if (lane == 0) s_cta = t;
     }
-    if (C > 1) {
+    if (NT == 256 && C > 1) {
         __syncthreads();
         cluster_wait();
         cg::cluster_group cl = cg::this_cluster();
@@ -391,7 +471,8 @@ __global__ __launch_bounds__(LP_NT, LP_OCC) void k_token_logprobs(const LogprobA
         cluster_wait();
         if (warp == 0) {
             LpStat t = s_stats[lane % C];
-            lp_join_lanes(t, C);
+            if (lane >= C) t.s = t.w = 0.0f;
+            lp_join_warp(t);
             if (lane == 0) s_cta = t;
         }
         if constexpr (TOP) {
@@ -409,34 +490,11 @@ __global__ __launch_bounds__(LP_NT, LP_OCC) void k_token_logprobs(const LogprobA
             for (int i = tid; i < C * a.n_top; i += LP_NT)
                 if (s_lists[i] >= bound && s_lists[i]) s_all[atomicAdd(&s_cnt[0], 1)] = s_lists[i];
             __syncthreads();
-            lp_rank(s_all, s_cnt[0], s_best, a.n_top, tid);
+            lp_rank<NT>(s_all, s_cnt[0], s_best, a.n_top, tid);
         }
     }
     __syncthreads();
-    const LpStat t = s_cta;
-    // s == 0: the row's mask leaves nothing; s NaN: a NaN or +inf, no distribution
-    const bool none = t.s == 0.0f, bad = t.s != t.s;
-    const float log_s = none ? 0.0f : logf(t.s), nan = __int_as_float(0x7fffffff);
-    if (tid == 0 && a.entropy) a.entropy[row] = none ? 0.0f : (bad ? nan : log_s - t.w / t.s);
-    for (int64_t j = tid; j < a.n_targets; j += LP_NT) {
-        const int64_t v = a.targets[row * a.n_targets + j];
-        float r = 0.0f;  // a negative target is no token
-        if (v >= a.V) {
-            atomicOr(a.err, PI_DEVERR_INDEX);
-            r = nan;
-        } else if (v >= 0) {
-            const float xt = lp_float(x[v]);
-            r = none ? -INFINITY : (bad ? nan : (xt - t.m) - log_s);
-        }
-        a.logp[row * a.n_targets + j] = r;
-    }
-    if constexpr (TOP) {
-        if (tid < a.n_top) {
-            const uint64_t k = bad ? 0 : s_best[tid];
-            a.top_ids[row * a.n_top + tid] = k ? (int32_t)lp_key_index(k) : -1;
-            a.top_logp[row * a.n_top + tid] = bad ? nan : (k ? (lp_key_value(k) - t.m) - log_s : -INFINITY);
-        }
-    }
+    answer(s_cta, tid, LP_NT);
 }
 
 // Clusters of more than 8 CTAs need the kernel's consent, once per kernel and device.
@@ -451,14 +509,17 @@ cudaError_t allow_wide_cluster(const void* fn, int device) {
     return e;
 }
 
-template <typename ET>
+template <typename ET, int NT>
 cudaError_t launch_logprobs(pi_ctx* ctx, const LogprobArgs& a, cudaStream_t st) {
-    auto kern = a.n_top > 0 ? k_token_logprobs<ET, true> : k_token_logprobs<ET, false>;
+    auto kern = a.n_top > 0 ? k_token_logprobs<ET, true, NT> : k_token_logprobs<ET, false, NT>;
     if (a.C > 8)
         if (cudaError_t e = allow_wide_cluster((const void*)kern, ctx->device)) return e;
+    // always raised: static and dynamic shared memory together pass the default of 48 KB
+    pi_smem_attr((const void*)kern, 64 * 1024);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.T * a.C));
-    cfg.blockDim = dim3(LP_NT);
+    cfg.blockDim = dim3(NT);
+    cfg.dynamicSmemBytes = lp_ring<NT>() * NT * 16;
     cfg.stream = st;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -467,6 +528,10 @@ cudaError_t launch_logprobs(pi_ctx* ctx, const LogprobArgs& a, cudaStream_t st) 
     cfg.attrs = at;
     cfg.numAttrs = a.C > 1 ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kern, a);
+}
+template <typename ET>
+cudaError_t launch_rows(pi_ctx* ctx, const LogprobArgs& a, bool warp_rows, cudaStream_t st) {
+    return warp_rows ? launch_logprobs<ET, 32>(ctx, a, st) : launch_logprobs<ET, 256>(ctx, a, st);
 }
 
 int token_logprobs(pi_ctx* ctx, const void* logits, int32_t dtype, int64_t T, int64_t V, int64_t ld,
@@ -485,13 +550,15 @@ int token_logprobs(pi_ctx* ctx, const void* logits, int32_t dtype, int64_t T, in
     if ((uintptr_t)logits % es) return pi_set_error(ctx, PI_ERR_ARG, "logprobs: logits are not aligned to their type");
     PiDeviceGuard dev(ctx->device);
     LogprobArgs a{logits, T, V, ld, targets, n_targets, n_top, 1, logp, entropy, top_ids, top_logp, ctx->dev_err};
-    // CTAs of a row: as long as all of the grid's run at once and each has two loads a thread
     const int64_t nvec = V * es / 16, sms = ctx->sm_count > 0 ? ctx->sm_count : 148;
-    while (a.C < LP_MAXC && T * a.C * 2 <= LP_OCC * sms && nvec >= (int64_t)a.C * 2 * 2 * LP_NT) a.C *= 2;
+    // A warp a row from eight rows per SM on. Below, 256 threads a row, and as many CTAs to it as
+    // still run all at once with two loads a thread each.
+    const bool warp_rows = T >= 8 * sms;
+    while (!warp_rows && a.C < LP_MAXC && T * a.C * 2 <= lp_occ<256>() * sms && nvec >= (int64_t)a.C * 2 * 2 * 256) a.C *= 2;
     PiProfScope ps(ctx, st, "k_token_logprobs");
-    const cudaError_t e = dtype == PI_QT_F32   ? launch_logprobs<float>(ctx, a, st)
-                          : dtype == PI_QT_F16 ? launch_logprobs<__half>(ctx, a, st)
-                                               : launch_logprobs<__nv_bfloat16>(ctx, a, st);
+    const cudaError_t e = dtype == PI_QT_F32   ? launch_rows<float>(ctx, a, warp_rows, st)
+                          : dtype == PI_QT_F16 ? launch_rows<__half>(ctx, a, warp_rows, st)
+                                               : launch_rows<__nv_bfloat16>(ctx, a, warp_rows, st);
     return pi_cuda_check(ctx, e, "logprobs");
 }
 

@@ -120,7 +120,8 @@ def test_refuses_without_a_gpu():
 @pytest.mark.parametrize("T,V,n_top,K,pad", [
     (1, 1, 1, 1, 0), (1, 2, 3, 2, 1), (3, 7, 32, 1, 0), (2, 31, 5, 0, 3), (5, 257, 32, 3, 2), (1, 1024, 1, 1, 0),
     (4, 4097, 20, 1, 5), (149, 1000, 4, 2, 0), (37, 32003, 8, 1, 1), (1, 151936, 20, 1, 0), (2, 151936, 32, 4, 0),
-    (1, 262144, 32, 1, 7), (300, 5000, 0, 1, 0), (700, 3001, 2, 1, 0)])
+    (1, 262144, 32, 1, 7), (300, 5000, 0, 1, 0), (700, 3001, 2, 1, 0), (1200, 1, 1, 1, 0), (1300, 37, 32, 2, 1),
+    (1184, 1031, 20, 1, 3), (1201, 9001, 1, 1, 0), (1500, 700, 0, 3, 0), (1190, 6000, 5, 0, 8)])
 def test_against_definition(dtype, T, V, n_top, K, pad):
     x = _logits(T, V, dtype, 7 * T + V, pad)
     rng = np.random.default_rng(T + V)
@@ -149,6 +150,10 @@ def test_ties_take_the_lowest_index(dtype, V):
             torch.where(i == V - 1, 1.0, 0.0), torch.where(i % 1024 == 5, 3.0, 0.5)]
     _check(torch.stack(rows).to(getattr(torch, dtype)), None, 20)
     _check(torch.stack(rows).to(getattr(torch, dtype)), None, 1)
+    if V <= 3000:  # as many rows as give each one warp
+        many = torch.stack(rows).to(getattr(torch, dtype)).repeat(150, 1)
+        _check(many, None, 20)
+        _check(many, None, 1)
 
 
 @pytest.mark.gpu
@@ -169,6 +174,9 @@ def test_masks(dtype, lowest):
     keep[3, :3] = True
     x = torch.where(keep, x, torch.full_like(x, low))
     tg = np.tile(np.array([0, 1, 2, V - 1]), (8, 1))
+    few = x[:, :1500].repeat(150, 1)  # a warp a row
+    few[3::8, :1497] = low
+    _check(few, None, 20)
     r = _check(x, tg, 20)
     if not lowest:
         assert float(r.entropy[1]) == 0.0 and (r.top_ids[1] == -1).all() and torch.isneginf(r.logp[1]).all()
@@ -187,6 +195,8 @@ def test_rows_without_a_distribution(V):
     x[4] = float("-inf")
     x[4, 17] = float("nan")
     x[5] = torch.finfo(torch.float32).max  # the largest finite value is a value
+    if V == 100:
+        _check(x.repeat(180, 1), np.zeros((1260, 1), np.int64), 3)  # a warp a row
     r = _check(x, np.zeros((7, 1), np.int64), 3)
     assert torch.isnan(r.entropy[1:5]).all() and (r.top_ids[1:5] == -1).all()
     assert not torch.isnan(r.entropy[[0, 5, 6]]).any()
