@@ -9,9 +9,8 @@
 // token's largest), block dots of the integer nibbles in f32, one fused multiply-add with
 // d_w per block. The adapters' products are f32 sums over unquantised x.
 //
-// Two launches: k_proj_prep (activations in the matrix instructions' fragment order, and
-// h_t = s_a A_a x_t), then k_proj_gemm (W's products, B_a h_t added to each output as it
-// is stored).
+// Up to three launches: k_proj_prep (activations in the matrix instructions' fragment order,
+// and h_t = s_a A_a x_t), k_proj_gemm (W's products), k_proj_adapters (B_a h_t added).
 #include "pi_common.cuh"
 #include "pi_internal.h"
 
@@ -160,14 +159,6 @@ PI_DEV uint32_t to_tf32(float v) {
     return r;
 }
 
-// Within a chunk the columns are ordered by adapter, those without one first, so that an
-// n-tile holds few adapters: the column of a token is the number of tokens of its chunk
-// with a smaller (adapter, token). Columns behind the last token keep their places.
-PI_DEV int lora_key(const LoraArgs& L, int64_t t) {
-    const int a = L.ids[t];
-    return a < 0 || a >= L.n ? -1 : a;
-}
-
 // ---------------------------------------------------------------------------
 // k_proj_prep: CTAs 0..T-1 put one token's activations in fragment order; the CTAs after
 // them compute h, four warps per token and four rank rows (each warp a quarter of the
@@ -190,19 +181,7 @@ __global__ __launch_bounds__(PREP_T) void k_proj_prep(const float* __restrict__ 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (blockIdx.x < T) {
         const int64_t t = blockIdx.x, chunk = t / (8 * NT), c0 = chunk * (8 * NT);
-        int col = (int)(t - c0);
-        if (L.ids) {
-            const int mine = lora_key(L, t), j = col;
-            col = 0;
-            for (int q = 0; q < 8 * NT; q += 32) {
-                bool before = false;
-                if (q + lane < 8 * NT && c0 + q + lane < T) {
-                    const int o = lora_key(L, c0 + q + lane);
-                    before = o < mine || (o == mine && q + lane < j);
-                }
-                col += __popc(__ballot_sync(0xffffffffu, before));
-            }
-        }
+        const int col = (int)(t - c0);
         const int g = col & 7;
         const float* xr = x + t * n_in;
         uint8_t* xo = xf + (chunk * units * NT + (col >> 3)) * xunit_bytes<QT>();
@@ -326,9 +305,7 @@ struct ProjArgs {
     const uint8_t* w;
     const uint8_t* xf;
     const float* xs;
-    const float* h;
     float* y;
-    LoraArgs L;
     int64_t T, n_out, units, tiles;
     int ks;      // CTAs that share the blocks of their rows
     int cu;      // units of a part that are staged together
@@ -392,16 +369,10 @@ constexpr int RING = 4;  // units a warp holds or has in flight (4 KB of Q8_0 we
 // CTA's warps share, double-buffered where a part does not fit. Splitting over CTAs rather
 // than over a CTA's warps keeps 128 rows to every staged fragment (n_out 12288, T 16, Q4_0:
 // 54 us with the blocks split over the warps, 36 over a cluster).
-//
-// Adapters: for every (adapter, n-tile) that meet, one product of the adapter's rows of B
-// (exact in tf32 for f16 and bf16 weights, two tf32 terms for f32 ones) with h in two tf32
-// terms on the tensor cores; a column takes it only where its token has that adapter, so
-// an adapter's NaN stays with its requests.
 template <int QT, int NT>
 __global__ __launch_bounds__(GEMM_T, 2) void k_proj_gemm(const ProjArgs p) {
     constexpr int XU = xunit_bytes<QT>(), UB = unit_bytes<QT>(), NC = 8 * NT, D = RING;
     extern __shared__ __align__(16) uint8_t s_x[];  // [2][cu][NT] fragment units, then the sums
-    __shared__ int s_key[NC], s_id[NC], s_rank[NC], s_tok[NC], s_pair[NC], s_npair;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, i4 = lane & 3;
     const int ks = p.ks, part = (int)(blockIdx.x % ks);
     const int64_t tile = (int64_t)(blockIdx.x / ks) * GEMM_W + warp;
@@ -432,39 +403,6 @@ __global__ __launch_bounds__(GEMM_T, 2) void k_proj_gemm(const ProjArgs p) {
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     stage(0);
-    if (p.L.ids) {
-        for (int j = tid; j < ncol; j += GEMM_T) s_key[j] = lora_key(p.L, t0 + j);
-        __syncthreads();
-        for (int j = tid; j < NC; j += GEMM_T) {
-            int col = j, a = -1, rank = 0;
-            if (j < ncol) {
-                a = s_key[j];
-                col = 0;
-                for (int q = 0; q < ncol; ++q) col += s_key[q] < a || (s_key[q] == a && q < j);
-                if (a >= 0) lora_of(p.L, t0 + j, &rank);
-            }
-            s_id[col] = a;
-            s_rank[col] = rank;
-            s_tok[col] = j;
-        }
-        __syncthreads();
-        if (warp == 0) {  // the (adapter, n-tile) pairs, each by its first column
-            int n = 0;
-            for (int q = 0; q < NC; q += 32) {
-                const int j = q + lane;
-                const bool start = j < NC && s_id[j] >= 0 && s_rank[j] > 0 && (j >> 3) % ks == part &&
-                                   ((j & 7) == 0 || s_id[j - 1] != s_id[j]);
-                const uint32_t b = __ballot_sync(0xffffffffu, start);
-                if (start) s_pair[n + __popc(b & ((1u << lane) - 1u))] = j;
-                n += __popc(b);
-            }
-            if (lane == 0) s_npair = n;
-        }
-    } else {
-        for (int j = tid; j < NC; j += GEMM_T) s_tok[j] = j;
-        if (tid == 0) s_npair = 0;
-    }
-
     uint64_t sum[NT][2];  // pairs of neighbouring columns, rows g and g + 8
 #pragma unroll
     for (int n = 0; n < NT; ++n) sum[n][0] = sum[n][1] = 0;
@@ -582,123 +520,11 @@ __global__ __launch_bounds__(GEMM_T, 2) void k_proj_gemm(const ProjArgs p) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const int u = n * 8 + 2 * i4;
-            const float su = u < ncol ? p.xs[t0 + s_tok[u]] : 0.0f, sv = u + 1 < ncol ? p.xs[t0 + s_tok[u + 1]] : 0.0f;
+            const float su = u < ncol ? p.xs[t0 + u] : 0.0f, sv = u + 1 < ncol ? p.xs[t0 + u + 1] : 0.0f;
             acc[n][0] *= su;
             acc[n][1] *= sv;
             acc[n][2] *= su;
             acc[n][3] *= sv;
-        }
-    }
-    const int npair = s_npair;
-    if (npair) {
-        const bool f32 = p.L.dtype == PI_QT_F32, f16 = p.L.dtype == PI_QT_F16;
-        const int es = f32 ? 4 : 2;
-        const uint8_t* bt = reinterpret_cast<const uint8_t*>(p.L.b) + (tile * 16 + g) * p.L.R * es;
-        const int64_t per_adapter = p.n_out * p.L.R * es, eight = (int64_t)8 * p.L.R * es;
-        struct Item {
-            uint4 b[2];   // four rank entries of rows g and g + 8 as they are stored
-            float4 h[2];  // h of the lane's column, large and small terms
-        } cur, nxt;
-        auto fetch = [&](Item& it, int i, int r0) {
-            const int j = s_pair[i], a = s_id[j], r = r0 + 4 * i4, col = (j & ~7) + g;
-            const bool in = r < s_rank[j];
-            const uint8_t* bp = bt + a * per_adapter + r * es;
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                it.b[k] = make_uint4(0, 0, 0, 0);
-                if (in && (tile * 16 + g) + 8 * k < p.n_out) {
-                    if (f32) {
-                        it.b[k] = __ldg(reinterpret_cast<const uint4*>(bp + k * eight));
-                    } else {
-                        const uint2 v = __ldg(reinterpret_cast<const uint2*>(bp + k * eight));
-                        it.b[k].x = v.x;
-                        it.b[k].y = v.y;
-                    }
-                }
-            }
-            it.h[0] = it.h[1] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (in && s_id[col] == a) {
-                const float4* hp = reinterpret_cast<const float4*>(p.h + ((t0 + s_tok[col]) * p.L.R + r) * 2);
-                it.h[0] = hp[0];
-                it.h[1] = hp[1];
-            }
-        };
-        float c[4] = {0.f, 0.f, 0.f, 0.f};
-        int i = 0, r0 = 0;
-        fetch(cur, 0, 0);
-        while (i < npair) {
-            const int j = s_pair[i], rank = s_rank[j];
-            const bool last = r0 + 16 >= rank;
-            const int ni = last ? i + 1 : i, nr = last ? 0 : r0 + 16;
-            if (ni < npair) fetch(nxt, ni, nr);
-            const int left = rank - r0 - 4 * i4;  // rank entries of this lane's four that count
-            const uint32_t* hb = reinterpret_cast<const uint32_t*>(&cur.h[0]);
-            const uint32_t* hs = reinterpret_cast<const uint32_t*>(&cur.h[1]);
-            uint32_t big[2][4], small[2][4];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const uint4 v = cur.b[k];
-                float f[4];
-                if (f32) {
-                    f[0] = __uint_as_float(v.x);
-                    f[1] = __uint_as_float(v.y);
-                    f[2] = __uint_as_float(v.z);
-                    f[3] = __uint_as_float(v.w);
-                } else if (f16) {
-                    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&v.x));
-                    const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
-                    f[0] = x.x;
-                    f[1] = x.y;
-                    f[2] = y.x;
-                    f[3] = y.y;
-                } else {
-                    f[0] = __uint_as_float(v.x << 16);
-                    f[1] = __uint_as_float(v.x & 0xffff0000u);
-                    f[2] = __uint_as_float(v.y << 16);
-                    f[3] = __uint_as_float(v.y & 0xffff0000u);
-                }
-#pragma unroll
-                for (int q = 1; q < 4; ++q)
-                    if (q >= left) f[q] = 0.0f;  // entry 0 past the rank was not loaded
-#pragma unroll
-                for (int q = 0; q < 4; ++q) big[q >> 1][k + 2 * (q & 1)] = __float_as_uint(f[q]);
-            }
-            if (f32) {
-#pragma unroll
-                for (int s = 0; s < 2; ++s)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const float f = __uint_as_float(big[s][q]);
-                        big[s][q] = to_tf32(f);
-                        small[s][q] = to_tf32(f - __uint_as_float(big[s][q]));
-                    }
-                mma_tf32(c, small[0], hb[0], hb[1]);
-                mma_tf32(c, small[1], hb[2], hb[3]);
-            }
-            mma_tf32(c, big[0], hs[0], hs[1]);
-            mma_tf32(c, big[1], hs[2], hs[3]);
-            mma_tf32(c, big[0], hb[0], hb[1]);
-            mma_tf32(c, big[1], hb[2], hb[3]);
-            if (last) {
-                const int n0 = j >> 3, a = s_id[j];
-                const bool u0 = s_id[n0 * 8 + 2 * i4] == a, u1 = s_id[n0 * 8 + 2 * i4 + 1] == a;
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-                    if (n == n0) {
-                        if (u0) {
-                            acc[n][0] += c[0];
-                            acc[n][2] += c[2];
-                        }
-                        if (u1) {
-                            acc[n][1] += c[1];
-                            acc[n][3] += c[3];
-                        }
-                    }
-                c[0] = c[1] = c[2] = c[3] = 0.0f;
-            }
-            cur = nxt;
-            i = ni;
-            r0 = nr;
         }
     }
     const int64_t row = tile * 16 + g;
@@ -709,10 +535,183 @@ __global__ __launch_bounds__(GEMM_T, 2) void k_proj_gemm(const ProjArgs p) {
         for (int e = 0; e < 2; ++e) {
             const int col = n * 8 + 2 * i4 + e;
             if (col >= ncol) continue;
-            float* y = p.y + (t0 + s_tok[col]) * p.n_out + row;
+            float* y = p.y + (t0 + col) * p.n_out + row;
             if (row < p.n_out) y[0] = acc[n][e];
             if (row + 8 < p.n_out) y[8] = acc[n][2 + e];
         }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// k_proj_adapters: y_t += B_a h_t. In a chunk of 64 tokens those of one adapter, up to eight
+// together, are the columns of a product on the tensor cores (B exact in tf32 for f16 and
+// bf16, two tf32 terms for f32; h in two terms); a warp's step is two tiles of 16 rows of one
+// such group. A token is in one group only, so an adapter's NaN stays with its requests and
+// every sum has one owner.
+//
+// A kernel of its own costs a second pass over y (mostly from L2), but its loads are as deep as
+// the occupancy allows; in the epilogue of k_proj_gemm a warp went through the groups one memory
+// latency after another (64 tokens, 2048 -> 151936, Q8_0, 16 adapters of rank 16: 224 us
+// together, 168 apart, 130 without adapters; 16 tokens, 4096 -> 12288, Q4_0, rank 64: 35 / 30 /
+// 21). Bound there: latency and issue (60%), 123 MB from memory in 40 us.
+// ---------------------------------------------------------------------------
+constexpr int AD_T = 256;
+constexpr int AD_C = 64;  // tokens of a chunk
+constexpr int AD_U = 2;   // tiles of a warp's step
+constexpr int AD_CTAS = 3;  // of an SM; the grid is what runs at once, its warps stride over the steps
+
+template <bool F32>
+__global__ __launch_bounds__(AD_T, AD_CTAS) void k_proj_adapters(const LoraArgs L, const float* __restrict__ h, int64_t T,
+                                                        int64_t n_out, int steps, float* __restrict__ y) {
+    constexpr int ES = F32 ? 4 : 2;
+    __shared__ int s_key[AD_C], s_tok[AD_C];
+    __shared__ int4 s_group[AD_C];  // adapter, rank, first place in s_tok, tokens
+    __shared__ int s_groups;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, i4 = lane & 3;
+    const int64_t t0 = (int64_t)blockIdx.y * AD_C;
+    const int ncol = (int)min((int64_t)AD_C, T - t0);
+    // the kernels before this one have waited for what wrote the ids and weights before they let
+    // it start: only y is waited for
+    int rank = 0;
+    if (tid < AD_C) s_key[tid] = tid < ncol ? lora_of(L, t0 + tid, &rank) : -1;
+    __syncthreads();
+    if (tid < AD_C) {
+        const int a = rank > 0 ? s_key[tid] : -1;
+        int less = 0, before = 0, all = 0;
+        for (int q = 0; q < ncol; ++q) {
+            const int k = s_key[q];
+            less += k < a;
+            all += k == a;
+            before += k == a && q < tid;
+        }
+        const bool start = a >= 0 && (before & 7) == 0;
+        if (a >= 0) s_tok[less + before] = tid;
+        const uint32_t b = __ballot_sync(0xffffffffu, start);
+        if (tid == 0) s_groups = __popc(b);
+        asm volatile("bar.sync 1, 64;" ::: "memory");
+        const int at = (warp ? s_groups : 0) + __popc(b & ((1u << lane) - 1u));
+        asm volatile("bar.sync 1, 64;" ::: "memory");
+        if (start) s_group[at] = make_int4(a, rank, less + before, min(8, all - before));
+        if (tid == 32) s_groups += __popc(b);
+    }
+    __syncthreads();
+    const int groups = s_groups, stride = (int)gridDim.x * (AD_T / 32);
+    const bool f16 = L.dtype == PI_QT_F16;
+    const int64_t row_bytes = (int64_t)L.R * ES;
+    const uint8_t* bw = reinterpret_cast<const uint8_t*>(L.b) + 4 * i4 * ES;
+    pdl_wait();
+    pdl_trigger();
+    int group = 0, step = (int)blockIdx.x * (AD_T / 32) + warp;
+    while (true) {
+        while (step >= steps && group < groups) {
+            step -= steps;
+            ++group;
+        }
+        if (group >= groups) break;
+        const int64_t row0 = (int64_t)step * (16 * AD_U) + g;
+        const int rows = (int)min(n_out - row0, (int64_t)(16 * AD_U));  // from row0 on; may be 0 or less
+        const int4 gr = s_group[group];
+        const float* hp = h + ((t0 + s_tok[gr.z + min(g, gr.w - 1)]) * L.R + 4 * i4) * 2;
+        const uint8_t* b0 = bw + ((int64_t)gr.x * n_out + row0) * row_bytes;
+        int64_t off[2 * AD_U];  // rows behind the last are not stored: they may hold the last one's
+#pragma unroll
+        for (int k = 0; k < 2 * AD_U; ++k) off[k] = min(8 * k, rows - 1) * row_bytes;
+        float* yp[2];
+        bool on[2];
+        float old[2 * AD_U][2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            on[e] = 2 * i4 + e < gr.w;
+            yp[e] = y + (t0 + (on[e] ? s_tok[gr.z + 2 * i4 + e] : 0)) * n_out + row0;
+#pragma unroll
+            for (int k = 0; k < 2 * AD_U; ++k) old[k][e] = on[e] && 8 * k < rows ? yp[e][8 * k] : 0.0f;
+        }
+        float c[AD_U][4];
+#pragma unroll
+        for (int u = 0; u < AD_U; ++u) c[u][0] = c[u][1] = c[u][2] = c[u][3] = 0.0f;
+#pragma unroll 1
+        for (int r0 = 0; r0 < gr.y; r0 += 16) {
+            const int left = gr.y - r0 - 4 * i4;  // rank entries of this lane's four that count
+            float4 hl = make_float4(0.f, 0.f, 0.f, 0.f), hs = hl;  // large and small terms
+            uint4 v[2 * AD_U];
+#pragma unroll
+            for (int k = 0; k < 2 * AD_U; ++k) v[k] = make_uint4(0, 0, 0, 0);
+            if (left > 0) {
+                hl = *reinterpret_cast<const float4*>(hp + r0 * 2);
+                hs = *reinterpret_cast<const float4*>(hp + r0 * 2 + 4);
+#pragma unroll
+                for (int k = 0; k < 2 * AD_U; ++k) {
+                    if constexpr (F32) {
+                        const int4 w = ld_stream(b0 + off[k] + r0 * ES);
+                        v[k] = make_uint4(w.x, w.y, w.z, w.w);
+                    } else {
+                        uint2 w;
+                        asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];"
+                                     : "=r"(w.x), "=r"(w.y)
+                                     : "l"(b0 + off[k] + r0 * ES));
+                        v[k].x = w.x;
+                        v[k].y = w.y;
+                    }
+                }
+            }
+            uint32_t big[AD_U][2][4], small[AD_U][2][4];
+#pragma unroll
+            for (int k = 0; k < 2 * AD_U; ++k) {
+                float f[4];
+                if constexpr (F32) {
+                    f[0] = __uint_as_float(v[k].x);
+                    f[1] = __uint_as_float(v[k].y);
+                    f[2] = __uint_as_float(v[k].z);
+                    f[3] = __uint_as_float(v[k].w);
+                } else if (f16) {
+                    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v[k].x));
+                    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&v[k].y));
+                    f[0] = a.x;
+                    f[1] = a.y;
+                    f[2] = b.x;
+                    f[3] = b.y;
+                } else {
+                    f[0] = __uint_as_float(v[k].x << 16);
+                    f[1] = __uint_as_float(v[k].x & 0xffff0000u);
+                    f[2] = __uint_as_float(v[k].y << 16);
+                    f[3] = __uint_as_float(v[k].y & 0xffff0000u);
+                }
+                if (gr.y & 3) {  // the rank ends inside four entries; fours behind it were not loaded
+#pragma unroll
+                    for (int q = 1; q < 4; ++q)
+                        if (q >= left) f[q] = 0.0f;
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q) big[k >> 1][q >> 1][(k & 1) + 2 * (q & 1)] = __float_as_uint(f[q]);
+            }
+            const uint32_t h0 = __float_as_uint(hl.x), h1 = __float_as_uint(hl.y), h2 = __float_as_uint(hl.z),
+                           h3 = __float_as_uint(hl.w);
+#pragma unroll
+            for (int u = 0; u < AD_U; ++u) {
+                if constexpr (F32) {
+#pragma unroll
+                    for (int s = 0; s < 2; ++s)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const float f = __uint_as_float(big[u][s][q]);
+                            big[u][s][q] = to_tf32(f);
+                            small[u][s][q] = to_tf32(f - __uint_as_float(big[u][s][q]));
+                        }
+                    mma_tf32(c[u], small[u][0], h0, h1);
+                    mma_tf32(c[u], small[u][1], h2, h3);
+                }
+                mma_tf32(c[u], big[u][0], __float_as_uint(hs.x), __float_as_uint(hs.y));
+                mma_tf32(c[u], big[u][1], __float_as_uint(hs.z), __float_as_uint(hs.w));
+                mma_tf32(c[u], big[u][0], h0, h1);
+                mma_tf32(c[u], big[u][1], h2, h3);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int k = 0; k < 2 * AD_U; ++k)
+                if (on[e] && 8 * k < rows) yp[e][8 * k] = old[k][e] + c[k >> 1][(k & 1) * 2 + e];
+        step += stride;
     }
 }
 
@@ -946,10 +945,21 @@ int proj_forward(pi_ctx* ctx, const pi_proj* P, const float* x, int64_t T, const
     }
     {
         PiProfScope ps(ctx, st, "k_proj_gemm");
-        const ProjArgs a{P->w, B.xf, B.xs, B.h, y, L, T, P->n_out, P->units, P->tiles, 1, 1, 1, 0};
+        const ProjArgs a{P->w, B.xf, B.xs, y, T, P->n_out, P->units, P->tiles, 1, 1, 1, 0};
         const int64_t sms = ctx->sm_count > 0 ? ctx->sm_count : 148;
         const cudaError_t e = q8 ? dispatch_gemm<PI_QT_Q8_0>(P, a, NT, sms, st) : dispatch_gemm<PI_QT_Q4_0>(P, a, NT, sms, st);
         if (e != cudaSuccess) return pi_cuda_check(ctx, e, "projection");
+    }
+    if (bank) {
+        PiProfScope ps(ctx, st, "k_proj_adapters");
+        const int64_t sms = ctx->sm_count > 0 ? ctx->sm_count : 148, steps = (P->n_out + 16 * AD_U - 1) / (16 * AD_U);
+        const int64_t chunks = (T + AD_C - 1) / AD_C, most = std::min<int64_t>(T, AD_C) * steps;  // items of a chunk
+        const int64_t ctas = std::min((most + AD_T / 32 - 1) / (AD_T / 32), std::max<int64_t>(1, AD_CTAS * sms / chunks));
+        const dim3 grid((unsigned)ctas, (unsigned)chunks);
+        if (L.dtype == PI_QT_F32)
+            pi_pdl_launch(k_proj_adapters<true>, grid, dim3(AD_T), 0, st, L, B.h, T, P->n_out, (int)steps, y);
+        else
+            pi_pdl_launch(k_proj_adapters<false>, grid, dim3(AD_T), 0, st, L, B.h, T, P->n_out, (int)steps, y);
     }
     return pi_cuda_check(ctx, cudaGetLastError(), "projection") ? PI_ERR_CUDA : PI_OK;
 }
