@@ -29,7 +29,7 @@ namespace {
 constexpr int LP_U = 4;          // 16-byte loads of a step
 // NT threads work on a row together: 256, or one warp where there are rows for all SMs. What does
 // not shrink with the row (threshold, joins, ranking) is then paid by one warp instead of
-// eight: 2048 rows of 32000 bf16 take 38 us, with 256 threads a row 41.
+// eight: 2048 rows of 32000 bf16 take 36 us, with 256 threads a row 41.
 template <int NT>
 constexpr int lp_occ() { return NT == 256 ? 3 : 16; }  // CTAs of an SM
 template <int NT>
@@ -125,6 +125,31 @@ PI_DEV void lp_unpack(const int4& q, float* x) {
     }
 }
 
+// Keeps the n best of the cnt keys in buf, in order, P a lane; the n-th one's value (-inf where
+// there are fewer). A function of its own: it is rare, and the loop around it is to stay in
+// the instruction cache.
+template <int P>
+__device__ __noinline__ float lp_keep_best(uint64_t* buf, int cnt, int n, int lane) {
+    uint64_t k[P];
+#pragma unroll
+    for (int i = 0; i < P; ++i) k[i] = lane + 32 * i < cnt ? buf[lane + 32 * i] : 0;
+    __syncwarp();
+    const int keep = min(n, cnt);
+    uint64_t best = 0;
+#pragma unroll 1
+    for (int r = 0; r < keep; ++r) {
+        uint64_t mine = 0;
+#pragma unroll
+        for (int i = 0; i < P; ++i) mine = k[i] > mine ? k[i] : mine;
+        best = warp_max_key(mine);
+#pragma unroll
+        for (int i = 0; i < P; ++i) k[i] = k[i] == best ? 0 : k[i];  // keys are distinct
+        if (lane == 0) buf[r] = best;
+    }
+    __syncwarp();
+    return keep == n ? lp_key_value(best) : -INFINITY;
+}
+
 // The largest values a warp has seen so far: a shared buffer of keys, a count, and the
 // value a further one has to exceed. Once n values of lower index reach `thr`, a later
 // value that only ties cannot be among the n best, so the comparison is strict; `incl`
@@ -136,46 +161,31 @@ struct LpTop {
     float thr = -INFINITY;
     bool incl = false;
 
-    // keeps the n best of the buffer, in order
     PI_DEV void compact() {
-        if (cnt <= 64) keep_best<2>();
-        else keep_best<CAP / 32>();
-    }
-    template <int P>  // P keys a lane
-    PI_DEV void keep_best() {
-        uint64_t k[P];
-#pragma unroll
-        for (int i = 0; i < P; ++i) k[i] = lane + 32 * i < cnt ? buf[lane + 32 * i] : 0;
-        __syncwarp();
-        const int keep = min(n, cnt);
-        uint64_t best = 0;
-        for (int r = 0; r < keep; ++r) {
-            uint64_t mine = 0;
-#pragma unroll
-            for (int i = 0; i < P; ++i) mine = k[i] > mine ? k[i] : mine;
-            best = warp_max_key(mine);
-#pragma unroll
-            for (int i = 0; i < P; ++i) k[i] = k[i] == best ? 0 : k[i];  // keys are distinct
-            if (lane == 0) buf[r] = best;
-        }
-        cnt = keep;
-        if (keep == n) {
-            thr = fmaxf(thr, lp_key_value(best));
+        const float least = cnt <= 64 ? lp_keep_best<2>(buf, cnt, n, lane) : lp_keep_best<CAP / 32>(buf, cnt, n, lane);
+        if (cnt >= n) {
+            thr = fmaxf(thr, least);
             incl = false;
         }
-        __syncwarp();
+        cnt = min(cnt, n);
     }
     PI_DEV bool passes(float x) const { return x > thr || (incl && x == thr); }
-    // N values per lane, index i0 + j; every lane calls it
-    template <int N>
-    PI_DEV void add(const float* x, float vmax, uint32_t i0) {
+    // N values per lane, index i0 + j, once more in memory at `at`; every lane calls it
+    template <int N, typename ET>
+    PI_DEV void add(const float* x, float vmax, const ET* at, uint32_t i0) {
         if (!__any_sync(0xffffffffu, passes(vmax))) return;
         if (cnt + 32 * N > CAP) compact();
+        uint32_t mask = 0;
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const bool in = passes(x[j]);
-            const uint32_t b = __ballot_sync(0xffffffffu, in);
-            if (in) buf[cnt + __popc(b & ((1u << lane) - 1u))] = lp_key(x[j], i0 + j);
+        for (int j = 0; j < N; ++j) mask |= (uint32_t)passes(x[j]) << j;
+        while (true) {  // one value of every lane that has any, mostly a single time
+            const uint32_t b = __ballot_sync(0xffffffffu, mask != 0);
+            if (!b) break;
+            if (mask) {
+                const int j = __ffs(mask) - 1;
+                buf[cnt + __popc(b & ((1u << lane) - 1u))] = lp_key(lp_float(at[j]), i0 + j);
+                mask &= mask - 1;
+            }
             cnt += __popc(b);
         }
         __syncwarp();
@@ -308,7 +318,7 @@ __global__ __launch_bounds__(NT, lp_occ<NT>()) void k_token_logprobs(const Logpr
             if (v > m) raise(v);
             pair(v, -INFINITY);
         }
-        if constexpr (TOP) top.template add<1>(&v, v, (uint32_t)lane);
+        if constexpr (TOP) top.template add<1>(&v, v, x + lane, (uint32_t)lane);
     }
     // Loads go through a ring in shared memory, of which a thread reads only what it copied itself
     // (no barrier): 32 KB a CTA in flight. In registers 8 KB were (2048 rows of 32000 bf16: 47
@@ -331,16 +341,13 @@ __global__ __launch_bounds__(NT, lp_occ<NT>()) void k_token_logprobs(const Logpr
     for (int i = 0; i < LP_D; i += LP_U) request(v0 + i * step, i);
     bool first = true;
     for (; v0 - tid < nvec || first; v0 += LP_U * step) {
-        float f[LP_U][NV], vmax[LP_U], mx = -INFINITY;
+        float f[LP_U][NV], mx = -INFINITY;
         asm volatile("cp.async.wait_group %0;" ::"n"(LP_D / LP_U - 1) : "memory");
 #pragma unroll
         for (int u = 0; u < LP_U; ++u) {
             lp_unpack<ET>(v0 + u * step < nvec ? s_ring[(slot + u) * LP_NT + tid] : none, f[u]);  // behind the end: -inf
-            vmax[u] = lp_max<NV>(f[u]);
-            mx = fmaxf(mx, vmax[u]);
+            mx = fmaxf(mx, lp_max<NV>(f[u]));
         }
-        request(v0 + LP_D * step, slot);
-        slot = slot + LP_U == LP_D ? 0 : slot + LP_U;
         if constexpr (TOP) {
             if (first) {
                 if (a.n_top <= LP_W) {
@@ -383,11 +390,24 @@ __global__ __launch_bounds__(NT, lp_occ<NT>()) void k_token_logprobs(const Logpr
             for (int j = 0; j < NV; j += 2) pair(f[u][j], f[u][j + 1]);
         if constexpr (TOP) {
             if (__any_sync(0xffffffffu, top.passes(mx)))
-#pragma unroll
-                for (int u = 0; u < LP_U; ++u)
-                    top.template add<NV>(f[u], vmax[u], (uint32_t)(head + (v0 + u * step) * NV));
+// 16-bit types: a loop over values read once more, for the code to fit the instruction cache (600
+// rows of 32000 bf16, n = 8: 50 us unrolled, 31 so; f32, half as many values: 90 as a loop, 83)
+#pragma unroll (NV == 4 ? LP_U : 1)
+                for (int u = 0; u < LP_U; ++u) {
+                    const int4* at = &s_ring[(slot + u) * LP_NT + tid];
+                    const uint32_t i0 = (uint32_t)(head + (v0 + u * step) * NV);
+                    if constexpr (NV == 4) {
+                        top.template add<NV>(f[u], lp_max<NV>(f[u]), reinterpret_cast<const ET*>(at), i0);
+                    } else {
+                        float e[NV];
+                        lp_unpack<ET>(v0 + u * step < nvec ? *at : none, e);
+                        top.template add<NV>(e, lp_max<NV>(e), reinterpret_cast<const ET*>(at), i0);
+                    }
+                }
             top.incl = false;
         }
+        request(v0 + LP_D * step, slot);
+        slot = slot + LP_U == LP_D ? 0 : slot + LP_U;
         first = false;
     }
     if (edges) {
@@ -397,7 +417,7 @@ __global__ __launch_bounds__(NT, lp_occ<NT>()) void k_token_logprobs(const Logpr
             if (v > m) raise(v);
             pair(v, -INFINITY);
         }
-        if constexpr (TOP) top.template add<1>(&v, v, (uint32_t)i);
+        if constexpr (TOP) top.template add<1>(&v, v, x + i, (uint32_t)i);
     }
 
     const float2 ss = unpack2(s2), ww = unpack2(w2);
