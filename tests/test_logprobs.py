@@ -301,6 +301,33 @@ def test_streams_graphs_and_repeats():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("n_top", [1, 8, 32])
+def test_rising_rows_and_many_rows(dtype, n_top):
+    """Logits that rise along the row: every value is among the best so far, so that buffers fill
+    again and again; few rows, and more than eight for each SM."""
+    import torch
+
+    for T, V in ((3, 9001), (1300, 1500)):
+        up = torch.linspace(-3.0, 3.0, V, device="cuda").expand(T, V) + torch.arange(T, device="cuda")[:, None] % 5
+        _check(up.to(getattr(torch, dtype)), np.full(T, V - 1), n_top)
+
+
+@pytest.mark.gpu
+def test_first_call_of_a_shape_under_capture():
+    import torch
+
+    from powerinfer_x64_b200.logprobs import token_logprobs
+
+    x = torch.randn(2, 77777, device="cuda", dtype=torch.float16)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        r = token_logprobs(x, None, 11)
+    g.replay()
+    assert all(torch.equal(p, q) for p, q in zip(r, token_logprobs(x, None, 11)) if p is not None)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("qtype", [8, 0])
 def test_lm_head_logprobs(orc, qtype):
     """The resident LM head and the scores of its logits, as a server chains them."""

@@ -321,6 +321,71 @@ def test_scratch_arena_instead_of_a_workspace(orc):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_one_adapter_for_a_long_batch_and_empty_ones(orc, dtype):
+    """Groups of eight tokens over several chunks of 64, the same adapter everywhere; adapters of
+    rank 0 add nothing."""
+    import torch
+
+    from powerinfer_x64_b200.lora import AdapterBank, SharedProjection
+
+    rng = np.random.default_rng(14)
+    T, n_in, n_out, n, R = 201, 96, 47, 3, 20
+    raw, w = _weights(orc, n_out, n_in, 8, rng)
+    a, b, ranks, scales = _bank(rng, n, R, n_in, n_out, getattr(torch, dtype))
+    ranks[:] = R, 0, 3
+    x = rng.standard_normal((T, n_in)).astype(np.float32)
+    P, xd = SharedProjection(raw, 8, n_out, n_in), torch.from_numpy(x).cuda()
+    bank = AdapterBank(a.cuda(), b.cuda(), ranks=torch.from_numpy(ranks).cuda(), scales=torch.from_numpy(scales).cuda())
+    for ids in (np.zeros(T, np.int32), np.ones(T, np.int32), np.arange(T, dtype=np.int32) % 3):
+        y = P.forward(xd, bank, torch.from_numpy(ids).cuda())
+        _close(y, *_reference(orc, x, w, 8, a, b, ranks, scales, ids))
+    assert torch.equal(P.forward(xd, bank, torch.ones(T, dtype=torch.int32, device="cuda")), P.forward(xd))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["a", "b"])
+def test_an_adapters_nan_stays_with_its_tokens(orc, which):
+    import torch
+
+    from powerinfer_x64_b200.lora import AdapterBank, SharedProjection
+
+    rng = np.random.default_rng(15)
+    raw, _ = _weights(orc, 70, 64, 8, rng)
+    a, b = torch.randn(4, 9, 64, device="cuda"), torch.randn(4, 70, 9, device="cuda")
+    ids = torch.tensor([0, 1, 2, 3, -1, 2, 1, 0, 3, 3, 2], dtype=torch.int32, device="cuda")
+    x = torch.randn(11, 64, device="cuda")
+    P = SharedProjection(raw, 8, 70, 64)
+    want = P.forward(x, AdapterBank(a, b), ids)
+    (a if which == "a" else b)[2, 5 if which == "a" else slice(None), 4] = float("nan")
+    y = P.forward(x, AdapterBank(a, b), ids)
+    hit = ids == 2
+    assert torch.isnan(y[hit]).all() and torch.equal(y[~hit], want[~hit])
+
+
+@pytest.mark.gpu
+def test_first_call_of_a_shape_under_capture(orc):
+    """What a shape's first call finds out (launch plan, workspace) it may find out while captured."""
+    import torch
+
+    from powerinfer_x64_b200.lora import AdapterBank, SharedProjection
+
+    rng = np.random.default_rng(16)
+    raw, _ = _weights(orc, 900, 192, 2, rng)
+    P = SharedProjection(raw, 2, 900, 192)
+    bank = AdapterBank(torch.randn(2, 8, 192, device="cuda"), torch.randn(2, 900, 8, device="cuda"))
+    x, ids = torch.randn(21, 192, device="cuda"), torch.arange(21, device="cuda").int() % 3 - 1
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = P.forward(x, bank, ids)
+    g.replay()
+    first = y.clone()
+    bank.set(1, torch.randn(5, 192), torch.randn(900, 5), 2.0)  # the graph reads the bank as it is at each replay
+    g.replay()
+    assert torch.equal(y, P.forward(x, bank, ids)) and not torch.equal(y, first)
+
+
+@pytest.mark.gpu
 def test_projection_then_scores(orc):
     """A decode step's end: LM head with the requests' adapters, then the scores of its logits."""
     import torch

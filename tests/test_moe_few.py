@@ -288,3 +288,21 @@ def test_decode_step_of_all_three(orc):
     lp, ent, top, _ = scores(logits.double().cpu().numpy(), best.cpu().numpy(), 3)
     assert np.abs(r.logp.cpu().numpy() - lp).max() <= (V / 256 + 90) * U + 2.0 ** -20
     assert np.array_equal(r.top_ids.cpu().numpy(), top)
+
+
+@pytest.mark.gpu
+def test_first_call_of_a_layer_under_capture(orc):
+    import torch
+
+    d, f, E, k = 1024, 256, 24, 5
+    rng = np.random.default_rng(8)
+    L = _make(_layer(orc, rng, d, f, E, k, "gated", True), d, f, E, k)
+    x = torch.randn(3, d, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = L.forward(x, rmsnorm=True, path="fused")
+    for scale in (1.0, -0.5):
+        x.mul_(scale)
+        g.replay()
+        assert torch.equal(y, L.forward(x, rmsnorm=True, path="fused"))
+    L.ctx.sync_check()
