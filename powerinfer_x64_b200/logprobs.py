@@ -54,8 +54,8 @@ def token_logprobs(logits, targets=None, n_top: int = 0) -> TokenLogprobs:
     if n_top:
         if not 0 < n_top <= 32:
             raise PiError(PI_ERR_ARG, "logprobs: 0 <= n_top <= 32")
-        ids = torch.empty((T, n_top), dtype=torch.int32, device=dev)
-        top = torch.empty((T, n_top), dtype=torch.float32, device=dev)
+        ids = torch.empty(T, n_top, dtype=torch.int32, device=dev)
+        top = torch.empty(T, n_top, dtype=torch.float32, device=dev)
     if T:
         ctx = Context.of(dev.index)
         rc = lib().pi_token_logprobs(ctx.h, logits.data_ptr(), qt, T, V, ld, targets.data_ptr() if K else None, K,

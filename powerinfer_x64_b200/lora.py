@@ -113,7 +113,7 @@ class SharedProjection:
                 raise PiError(PI_ERR_ARG, f"projection: adapter_ids must be contiguous int32 [T] on {self.device}")
             desc, ids, rank = bank._desc, adapter_ids.data_ptr(), bank.rank
         if out is None:
-            out = torch.empty((T, n_out), dtype=torch.float32, device=self.device)
+            out = torch.empty(T, n_out, dtype=torch.float32, device=self.device)
         elif out.dtype != torch.float32 or out.shape != (T, n_out) or out.get_device() != dev or \
                 not out.is_contiguous():
             raise PiError(PI_ERR_ARG, f"projection: out must be contiguous f32 [T, {n_out}] on {self.device}")

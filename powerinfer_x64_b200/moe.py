@@ -129,7 +129,7 @@ class MoeLayer:
             raise PiError(PI_ERR_ARG, f"moe: x must be contiguous f32 [T, {d}] on cuda:{dev}")
         T = n // d
         if out is None:
-            out = torch.empty((T, d), dtype=torch.float32, device=x.device)
+            out = torch.empty(T, d, dtype=torch.float32, device=x.device)
         elif out.dtype != torch.float32 or out.get_device() != dev or not out.is_contiguous() or out.numel() != n:
             raise PiError(PI_ERR_ARG, f"moe: out must be contiguous f32 [T, {d}] on cuda:{dev}")
         L, flags = lib(), (PI_FWD_RMSNORM if rmsnorm else 0) | (PI_FWD_RESIDUAL if residual else 0)
