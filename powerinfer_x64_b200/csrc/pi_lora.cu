@@ -161,21 +161,21 @@ PI_DEV uint32_t to_tf32(float v) {
 
 // ---------------------------------------------------------------------------
 // k_proj_prep: CTAs 0..T-1 put one token's activations in fragment order; the CTAs after
-// them compute h, four warps per token and four rank rows (each warp a quarter of the
-// row: its loads are then one or two round trips to memory for usual widths). Padded
-// blocks of a row are zero; the columns of tokens behind the last one hold whatever the
-// buffer held, and no output reads them (a column of a product depends on it alone).
+// them compute h, S = 2, 4, 8 or 16 warps per token and four rank rows (a row's parts in turn, 256
+// values of each at a time: few tokens take many warps, whose loads are then one or two round
+// trips to memory). Padded blocks of a row are zero; the columns of tokens behind the last
+// one hold whatever the buffer held, and no output reads them (a column of a product depends
+// on it alone).
 // Q4_0 activations are scaled by a power of two per token, its reciprocal in xs [T].
 // ---------------------------------------------------------------------------
-constexpr int PREP_T = 256;
+constexpr int PREP_T = 512;
 constexpr int PREP_R = 4;   // rank rows of a unit
-constexpr int PREP_S = 4;   // warps of a unit
 
 template <int QT>
 __global__ __launch_bounds__(PREP_T) void k_proj_prep(const float* __restrict__ x, int64_t T, int64_t n_in,
                                                       int64_t units, int NT, uint8_t* __restrict__ xf,
                                                       float* __restrict__ xs, const LoraArgs L,
-                                                      float* __restrict__ h, uint32_t* err) {
+                                                      float* __restrict__ h, int S, uint32_t* err) {
     pdl_wait();
     pdl_trigger();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -251,8 +251,8 @@ __global__ __launch_bounds__(PREP_T) void k_proj_prep(const float* __restrict__ 
     // h[t][r] = scale * (A[a][r] . x[t]), zero from the rank on, as two tf32 terms: per unit
     // of four rank rows the four large terms, then the four small ones
     __shared__ float s_h[PREP_T / 32][PREP_R];
-    const int per = L.R / PREP_R, part = warp % PREP_S;
-    const int64_t unit = (blockIdx.x - T) * (PREP_T / 32 / PREP_S) + warp / PREP_S, t = unit / per;
+    const int per = L.R / PREP_R, part = warp % S;
+    const int64_t unit = (blockIdx.x - T) * (PREP_T / 32 / S) + warp / S, t = unit / per;
     const int r0 = (int)(unit % per) * PREP_R;
     int rank = 0, a = -1;
     if (t < T) a = lora_of(L, t, &rank);
@@ -262,7 +262,7 @@ __global__ __launch_bounds__(PREP_T) void k_proj_prep(const float* __restrict__ 
         const float* xr = x + t * n_in;
         const int64_t base = ((int64_t)a * L.R + r0) * n_in;
 #pragma unroll 4
-        for (int64_t k = part * 256 + lane * 8; k < n_in; k += 256 * PREP_S) {
+        for (int64_t k = part * 256 + lane * 8; k < n_in; k += 256 * S) {
             const float4 u = *reinterpret_cast<const float4*>(xr + k);
             const float4 v = *reinterpret_cast<const float4*>(xr + k + 4);
 #pragma unroll
@@ -288,8 +288,7 @@ __global__ __launch_bounds__(PREP_T) void k_proj_prep(const float* __restrict__ 
     __syncthreads();
     if (live && part == 0 && lane < PREP_R) {
         float s = 0.0f;
-#pragma unroll
-        for (int q = 0; q < PREP_S; ++q) s += s_h[warp + q][lane];
+        for (int q = 0; q < S; ++q) s += s_h[warp + q][lane];
         s = r0 + lane < rank ? s * (L.scales ? L.scales[a] : 1.0f) : 0.0f;
         const uint32_t big = to_tf32(s);
         float* o = h + (t * L.R + r0) * 2 + lane;
@@ -935,13 +934,19 @@ int proj_forward(pi_ctx* ctx, const pi_proj* P, const float* x, int64_t T, const
     const int NT = proj_chunk(T);
     {
         PiProfScope ps(ctx, st, "k_proj_prep");
-        const int64_t units = T * (R / PREP_R), per = PREP_T / 32 / PREP_S, grid = T + (units + per - 1) / per;
+        // the warps of a unit: many where there are few units (4 tokens, 11008 wide, rank 64: 29 us with
+        // 4, 25 with 8, 23 with 16; 16 tokens, 4096: 30.4 / 29.2), few where there are many (231 tokens,
+        // 640, rank 104: 71 with 4, 68 with 2), and none without 256 values of a row
+        const int64_t units = T * (R / PREP_R);
+        int S = units <= 128 ? 16 : (units <= 512 ? 8 : (units < 2048 ? 4 : 2));
+        while (S > 2 && S * 128 >= P->n_in) S /= 2;
+        const int64_t per = PREP_T / 32 / S, grid = T + (units + per - 1) / per;
         if (q8)
             pi_pdl_launch(k_proj_prep<PI_QT_Q8_0>, dim3((unsigned)grid), dim3(PREP_T), 0, st, x, T, P->n_in, P->units,
-                          NT, B.xf, B.xs, L, B.h, ctx->dev_err);
+                          NT, B.xf, B.xs, L, B.h, S, ctx->dev_err);
         else
             pi_pdl_launch(k_proj_prep<PI_QT_Q4_0>, dim3((unsigned)grid), dim3(PREP_T), 0, st, x, T, P->n_in, P->units,
-                          NT, B.xf, B.xs, L, B.h, ctx->dev_err);
+                          NT, B.xf, B.xs, L, B.h, S, ctx->dev_err);
     }
     {
         PiProfScope ps(ctx, st, "k_proj_gemm");
