@@ -551,7 +551,7 @@ __global__ __launch_bounds__(GEMM_T, 2) void k_proj_gemm(const ProjArgs p) {
 // A kernel of its own costs a second pass over y (mostly from L2), but its loads are as deep as
 // the occupancy allows; in the epilogue of k_proj_gemm a warp went through the groups one memory
 // latency after another (64 tokens, 2048 -> 151936, Q8_0, 16 adapters of rank 16: 224 us
-// together, 168 apart, 130 without adapters; 16 tokens, 4096 -> 12288, Q4_0, rank 64: 35 / 30 /
+// together, 167 apart, 130 without adapters; 16 tokens, 4096 -> 12288, Q4_0, rank 64: 35 / 30 /
 // 21). Bound there: latency and issue (60%), 123 MB from memory in 40 us.
 // ---------------------------------------------------------------------------
 constexpr int AD_T = 256;
