@@ -27,13 +27,15 @@ namespace cg = cooperative_groups;
 namespace {
 
 constexpr int LP_U = 4;          // 16-byte loads of a step
-// NT threads work on a row together: 256, or one warp where there are rows for all SMs. What does
-// not shrink with the row (threshold, joins, ranking) is then paid by one warp instead of
-// eight: 2048 rows of 32000 bf16 take 36 us, with 256 threads a row 41.
+// NT threads work on a row together: 256 (or a cluster of such CTAs), 64 from five rows per SM on,
+// one warp from eight. What does not shrink with the row (threshold, joins, ranking) is then
+// paid by fewer warps, and the CTAs fill the SMs in whole waves: 2048 rows of 32000 bf16 take 36 us
+// with a warp, 41 with 256 threads; 1000 rows of 128000 f32, n = 8: 107 us with 64, 121 with 256;
+// 700 rows, bf16: 34 with 64, 33 with 256.
 template <int NT>
-constexpr int lp_occ() { return NT == 256 ? 3 : 16; }  // CTAs of an SM
+constexpr int lp_occ() { return NT == 256 ? 3 : (NT == 64 ? 12 : 16); }  // CTAs of an SM
 template <int NT>
-constexpr int lp_ring() { return NT == 256 ? 8 : 12; }  // 16-byte loads a thread has in flight or at hand
+constexpr int lp_ring() { return NT == 32 ? 12 : 8; }  // 16-byte loads a thread has in flight or at hand
 constexpr int LP_MAXC = 16;      // CTAs of a cluster at most
 constexpr int LP_MAXTOP = 32;    // alternatives at most
 constexpr float LP_LOG2E = 1.4426950408889634f;
@@ -233,7 +235,7 @@ PI_DEV void lp_join_warp(LpStat& st) {
 template <typename ET, bool TOP, int NT>
 __global__ __launch_bounds__(NT, lp_occ<NT>()) void k_token_logprobs(const LogprobArgs a) {
     constexpr int LP_NT = NT, LP_W = NT / 32, LP_D = lp_ring<NT>();
-    constexpr int GROUP = NT == 256 ? 4 : 1, GROUPS = NT / GROUP;  // groups of lanes whose maxima give the threshold
+    constexpr int GROUP = NT == 32 ? 1 : (NT == 64 ? 2 : 4), GROUPS = NT / GROUP;  // groups of lanes whose maxima give the threshold
     constexpr int KEYS = NT == 256 ? LP_MAXC * LP_MAXTOP : 320;    // keys ranked together; one warp has no cluster
     constexpr int NV = 16 / (int)sizeof(ET);
     constexpr int CAP = 64 + 32 * NV;  // n kept after compact() and one load of every lane
@@ -433,7 +435,7 @@ __global__ __launch_bounds__(NT, lp_occ<NT>()) void k_token_logprobs(const Logpr
             if (i < warp) at += s_cnt[i];
             total += s_cnt[i];
         }
-        if (NT == 256 && total > NT) {
+        if (NT > 32 && total > 256) {
             __syncthreads();
             if (top.cnt > a.n_top) top.compact();
             if (lane == 0) s_cnt[warp] = top.cnt;
@@ -446,7 +448,7 @@ __global__ __launch_bounds__(NT, lp_occ<NT>()) void k_token_logprobs(const Logpr
         }
         for (int i = lane; i < top.cnt; i += 32) s_all[at + i] = top.buf[i];
         __syncthreads();
-        if ((NT == 32 || C == 1) && total <= 32) {  // few keys: the first warp ranks them, the others are done
+        if ((NT < 256 || C == 1) && total <= 32) {  // few keys: the first warp ranks them, the others are done
             if (warp != 0) return;
             const uint64_t k = lane < total ? s_all[lane] : 0;
             int r = 0;
@@ -550,8 +552,10 @@ cudaError_t launch_logprobs(pi_ctx* ctx, const LogprobArgs& a, cudaStream_t st) 
     return cudaLaunchKernelEx(&cfg, kern, a);
 }
 template <typename ET>
-cudaError_t launch_rows(pi_ctx* ctx, const LogprobArgs& a, bool warp_rows, cudaStream_t st) {
-    return warp_rows ? launch_logprobs<ET, 32>(ctx, a, st) : launch_logprobs<ET, 256>(ctx, a, st);
+cudaError_t launch_rows(pi_ctx* ctx, const LogprobArgs& a, int threads, cudaStream_t st) {
+    return threads == 32   ? launch_logprobs<ET, 32>(ctx, a, st)
+           : threads == 64 ? launch_logprobs<ET, 64>(ctx, a, st)
+                           : launch_logprobs<ET, 256>(ctx, a, st);
 }
 
 int token_logprobs(pi_ctx* ctx, const void* logits, int32_t dtype, int64_t T, int64_t V, int64_t ld,
@@ -571,14 +575,14 @@ int token_logprobs(pi_ctx* ctx, const void* logits, int32_t dtype, int64_t T, in
     PiDeviceGuard dev(ctx->device);
     LogprobArgs a{logits, T, V, ld, targets, n_targets, n_top, 1, logp, entropy, top_ids, top_logp, ctx->dev_err};
     const int64_t nvec = V * es / 16, sms = ctx->sm_count > 0 ? ctx->sm_count : 148;
-    // A warp a row from eight rows per SM on. Below, 256 threads a row, and as many CTAs to it as
-    // still run all at once with two loads a thread each.
-    const bool warp_rows = T >= 8 * sms;
-    while (!warp_rows && a.C < LP_MAXC && T * a.C * 2 <= lp_occ<256>() * sms && nvec >= (int64_t)a.C * 2 * 2 * 256) a.C *= 2;
+    // with 256 threads a row, as many CTAs to it as still run all at once with two loads a thread each
+    const int threads = T >= 8 * sms ? 32 : (T >= 5 * sms ? 64 : 256);
+    if (threads == 256)
+        while (a.C < LP_MAXC && T * a.C * 2 <= lp_occ<256>() * sms && nvec >= (int64_t)a.C * 2 * 2 * 256) a.C *= 2;
     PiProfScope ps(ctx, st, "k_token_logprobs");
-    const cudaError_t e = dtype == PI_QT_F32   ? launch_rows<float>(ctx, a, warp_rows, st)
-                          : dtype == PI_QT_F16 ? launch_rows<__half>(ctx, a, warp_rows, st)
-                                               : launch_rows<__nv_bfloat16>(ctx, a, warp_rows, st);
+    const cudaError_t e = dtype == PI_QT_F32   ? launch_rows<float>(ctx, a, threads, st)
+                          : dtype == PI_QT_F16 ? launch_rows<__half>(ctx, a, threads, st)
+                                               : launch_rows<__nv_bfloat16>(ctx, a, threads, st);
     return pi_cuda_check(ctx, e, "logprobs");
 }
 

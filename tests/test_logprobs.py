@@ -305,10 +305,10 @@ def test_streams_graphs_and_repeats():
 @pytest.mark.parametrize("n_top", [1, 8, 32])
 def test_rising_rows_and_many_rows(dtype, n_top):
     """Logits that rise along the row: every value is among the best so far, so that buffers fill
-    again and again; few rows, and more than eight for each SM."""
+    again and again; few rows, more than eight and more than five for each SM."""
     import torch
 
-    for T, V in ((3, 9001), (1300, 1500)):
+    for T, V in ((3, 9001), (1300, 1500), (800, 2500)):
         up = torch.linspace(-3.0, 3.0, V, device="cuda").expand(T, V) + torch.arange(T, device="cuda")[:, None] % 5
         _check(up.to(getattr(torch, dtype)), np.full(T, V - 1), n_top)
 
