@@ -196,6 +196,15 @@ def stream_ptr(stream=None):
     return _P(stream.cuda_stream) if hasattr(stream, "cuda_stream") else _P(stream)
 
 
+def torch_stream(stream, device: int):
+    """``stream`` (a torch stream or a raw cudaStream_t of ``device``) as a torch stream."""
+    import torch
+
+    if hasattr(stream, "cuda_stream"):
+        return stream
+    return torch.cuda.ExternalStream(int(stream), device=device)
+
+
 def raw_stream(device: int) -> int:
     """cudaStream_t of torch's current stream on ``device`` (without making a Stream object)."""
     import torch

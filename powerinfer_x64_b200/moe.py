@@ -18,7 +18,7 @@ import numpy as np
 
 from . import quant
 from ._lib import (PI_FWD_FAST_SUM, PI_FWD_FORCE_GEMM, PI_FWD_FORCE_GEMV, PI_FWD_RESIDUAL, PI_FWD_RMSNORM, PI_QT_F32, Context, PiError, PiMoeLayerDesc, PI_ERR_ARG, lib,
-                   ptr, raw_stream, stream_ptr)
+                   ptr, raw_stream, stream_ptr, torch_stream)
 
 
 def _torch():
@@ -103,9 +103,15 @@ class MoeLayer:
         order than "gemv"). fast: the Q8_0 prefill GEMM adds each block
         term with a fused multiply-add (PI_FWD_FAST_SUM; within the parity tolerance,
         not bit-identical).
+
+        stream (a torch stream or a raw cudaStream_t): where the work runs, with memory from
+        that stream's own pool; x and a given out are to be ready there.
         """
+        if stream is not None:
+            return self._on_stream(stream, self.forward, x, out, rmsnorm=rmsnorm, residual=residual, path=path,
+                                   fast=fast)
         if path == "fused":
-            return self._forward_fused(x, out, rmsnorm, residual, stream, fast)
+            return self._forward_fused(x, out, rmsnorm, residual, fast)
         torch = _torch()
         xd = quant._f32(x)
         T = xd.numel() // self.n_embd
@@ -116,10 +122,27 @@ class MoeLayer:
         flags = (PI_FWD_RMSNORM if rmsnorm else 0) | (PI_FWD_RESIDUAL if residual else 0)
         flags |= {"auto": 0, "gemv": PI_FWD_FORCE_GEMV, "gemm": PI_FWD_FORCE_GEMM}[path]
         flags |= PI_FWD_FAST_SUM if fast else 0
-        self.ctx.check(lib().pi_moe_forward(self.ctx.h, self.h, ptr(xd), T, ptr(out), flags, stream_ptr(stream)))
+        self.ctx.check(lib().pi_moe_forward(self.ctx.h, self.h, ptr(xd), T, ptr(out), flags, stream_ptr()))
         return out
 
-    def _forward_fused(self, x, out, rmsnorm, residual, stream, fast):
+    def _on_stream(self, stream, call, x, out, **kw):
+        """``call(x, out, **kw)`` with ``stream`` current: what it allocates and converts then comes
+        from the pool of the stream that works on it. A block of the caller's stream's pool may
+        still be in use by what was launched there before, which ``stream`` does not wait for."""
+        torch = _torch()
+        side, cur = torch_stream(stream, self.ctx.device), torch.cuda.current_stream(self.ctx.device)
+        with torch.cuda.stream(side):
+            r = call(x, out, **kw)
+        if side != cur:
+            for t in (x, out):  # the caller's memory, should the caller let go of it before the work is done
+                if quant._is_dev(t):
+                    t.record_stream(side)
+            for t in (r[0], *r[1].values()) if isinstance(r, tuple) else (r,):
+                if t is not out:  # the side stream's memory, which the caller goes on to use on its own
+                    t.record_stream(cur)
+        return r
+
+    def _forward_fused(self, x, out, rmsnorm, residual, fast):
         torch = _torch()
         if fast:
             raise PiError(PI_ERR_ARG, "moe: the fused path has no fast sum")
@@ -138,13 +161,8 @@ class MoeLayer:
             nbytes = self._fused_ws[T] = L.pi_moe_fused_workspace(self.h, T)
         # the caching allocator's memory: one workspace per call and per captured graph
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        if stream is None:
-            raw = raw_stream(dev)
-        else:
-            raw = stream.cuda_stream
-            ws.record_stream(stream)
         rc = L.pi_moe_forward_fused(self.ctx.h, self.h, x.data_ptr(), T, out.data_ptr(), flags,
-                                    ws.data_ptr() if nbytes else None, nbytes, raw)
+                                    ws.data_ptr() if nbytes else None, nbytes, raw_stream(dev))
         if rc:
             self.ctx.check(rc)
         return out
@@ -154,6 +172,9 @@ class MoeLayer:
         """``forward`` that also returns the routing it used: (out, dict(idx, gates,
         counts, offsets, perm)) as ``route`` returns them, computed on the
         (optionally RMS-normed) tokens the forward itself routed."""
+        if stream is not None:
+            return self._on_stream(stream, self.forward_routed, x, out, rmsnorm=rmsnorm, residual=residual,
+                                   path=path, fast=fast)
         torch = _torch()
         xd = quant._f32(x)
         T = xd.numel() // self.n_embd
@@ -172,7 +193,7 @@ class MoeLayer:
         flags |= PI_FWD_FAST_SUM if fast else 0
         self.ctx.check(lib().pi_moe_forward_routed(self.ctx.h, self.h, ptr(xd), T, ptr(out), flags, ptr(o["idx"]),
                                                    ptr(o["gates"]), ptr(o["counts"]), ptr(o["offsets"]),
-                                                   ptr(o["perm"]), stream_ptr(stream)))
+                                                   ptr(o["perm"]), stream_ptr()))
         return out, o
 
 
