@@ -397,7 +397,7 @@ __global__ __launch_bounds__(NT, lp_occ<NT>()) void k_token_logprobs(const Logpr
 #pragma unroll (NV == 4 ? LP_U : 1)
                 for (int u = 0; u < LP_U; ++u) {
                     const int4* at = &s_ring[(slot + u) * LP_NT + tid];
-                    const uint32_t i0 = (uint32_t)(head + (v0 + u * step) * NV);
+                    const uint32_t i0 = (uint32_t)head + (uint32_t)(v0 + u * step) * NV;  // behind the end: past 2^31
                     if constexpr (NV == 4) {
                         top.template add<NV>(f[u], lp_max<NV>(f[u]), reinterpret_cast<const ET*>(at), i0);
                     } else {
@@ -413,13 +413,13 @@ __global__ __launch_bounds__(NT, lp_occ<NT>()) void k_token_logprobs(const Logpr
         first = false;
     }
     if (edges) {
-        const int i = tail + lane;
-        const float v = i < a.V ? lp_float(x[i]) : -INFINITY;
-        if (i < a.V) {
+        const bool in = lane < (int)(a.V - tail);  // tail + lane may pass 2^31
+        const float v = in ? lp_float(x[(int64_t)tail + lane]) : -INFINITY;
+        if (in) {
             if (v > m) raise(v);
             pair(v, -INFINITY);
         }
-        if constexpr (TOP) top.template add<1>(&v, v, x + i, (uint32_t)i);
+        if constexpr (TOP) top.template add<1>(&v, v, x + (int64_t)tail + lane, (uint32_t)tail + lane);
     }
 
     const float2 ss = unpack2(s2), ww = unpack2(w2);
