@@ -201,9 +201,12 @@ int pi_moe_forward_routed(pi_ctx* ctx, pi_moe_layer* layer, const float* x, int6
                           int32_t* idx, float* gates, int32_t* counts, int32_t* offsets, int32_t* perm, void* stream);
 
 /* pi_moe_forward for a few tokens in two kernels (model/mod.rs:1239-1633): a decode batch
- * of T <= 16 tokens through a Q4_0 layer that holds all its experts. Routing is that of
- * pi_moe_route bit for bit; outputs equal pi_moe_forward's to f32 rounding (block sums in
- * another order). flags: PI_FWD_RMSNORM | PI_FWD_RESIDUAL. x and out 16-byte aligned; out
+ * of T <= 16 tokens through a Q4_0 layer that holds all its experts. The experts chosen are
+ * those of pi_moe_route bit for bit, gates equal to f32 rounding. Expert products are exact
+ * sums over blocks of 32 inputs held in fixed point: an input (and each value of the hidden
+ * row) is kept in f32 or within 2^-22 of one that four of its block reach a 32nd of, so
+ * within 2^-17 of the block's fourth largest magnitude; NaN and infinities act as in f32.
+ * flags: PI_FWD_RMSNORM | PI_FWD_RESIDUAL. x and out 16-byte aligned; out
  * may be x. workspace: pi_moe_fused_workspace(layer, T) bytes, 256-byte aligned, that
  * nothing else uses until the call's work is done (two captured graphs need one each);
  * NULL: the stream's scratch arena (pi_ctx_reserve before a capture). The second kernel

@@ -10,6 +10,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -34,7 +35,7 @@ def build(verbose: bool = False) -> Path:
     OBJ.mkdir(exist_ok=True)
     LIB_DIR.mkdir(exist_ok=True)
     hm = _headers_mtime()
-    objs = []
+    objs, todo = [], []
     for src in sorted(CSRC.glob("*.cu")):
         obj = OBJ / (src.stem + ".o")
         objs.append(obj)
@@ -43,7 +44,9 @@ def build(verbose: bool = False) -> Path:
         cmd = [NVCC, *ARCH, *FLAGS, "-c", str(src), "-o", str(obj)]
         if verbose:
             print(" ".join(cmd), file=sys.stderr)
-        subprocess.run(cmd, check=True)
+        todo.append(cmd)
+    with ThreadPoolExecutor(os.cpu_count()) as pool:
+        list(pool.map(lambda cmd: subprocess.run(cmd, check=True), todo))
     if not LIB.exists() or LIB.stat().st_mtime < max(o.stat().st_mtime for o in objs):
         cmd = [NVCC, *ARCH, "-shared", "-o", str(LIB), *map(str, objs), "-lcudart"]
         if verbose:

@@ -17,8 +17,10 @@
 // 958-969). Here 32 inputs that share a weight scale become fixed-point numbers of 22 bits
 // below their largest, held as three int8 terms, so a block's dot with the nibbles is three
 // exact integer dots (dp4a: 1.1 instructions a weight and token, against 2.4 for decoding
-// nibbles to f32), and one f32 multiply-add per block follows. An input is then within 2^-22 of
-// its block's largest, which moves a sum by no more than f32 products and sums do.
+// nibbles to f32), and one f32 multiply-add per block follows. Values that stand far above the
+// rest of their block are held apart in f32 and multiplied one by one: every other value is then
+// within 2^-22 of one that four of its 32 reach a 32nd of, so within 2^-17 of the block's
+// fourth largest, and an outlier whose weight is 0 costs its neighbours nothing.
 //
 // Bound: the bytes of the experts that the tokens use; for a token or two the latency of the
 // chain (two launches, the barrier and four dependent trips to memory). k_few_experts is launched cooperatively: its
@@ -29,6 +31,7 @@
 
 #include <algorithm>
 #include <exception>
+#include <type_traits>
 
 namespace {
 
@@ -36,40 +39,108 @@ constexpr int FEW_T = 16;  // tokens at most
 
 // ---------------------------------------------------------------------------
 // Fixed-point blocks. 32 values in eight lanes, four each: with 2^e the power of two that
-// brings the largest into [2^21, 2^22), X = rint(x 2^e) = 65536 q1 + 256 q2 + q3, each q an
-// int8. A block is 28 words: [term][word of eight elements][even elements, odd elements], as
-// the nibbles of a Q4_0 word fall apart (low: even, high: odd), then the scale 2^-e / 16
-// (nibbles come shifted by four bits), then padding that keeps the lanes' 16-byte reads of
-// neighbouring blocks in distinct banks. A NaN or infinity makes the block's scale NaN.
+// brings the largest of those not held apart into [2^21, 2^22), X = rint(x 2^e) = 65536 q1 + 256
+// q2 + q3, each q an int8. A block is 28 words: [term][word of eight elements][even elements, odd
+// elements], as the nibbles of a Q4_0 word fall apart (low: even, high: odd), then the scale
+// 2^-e / 16 (nibbles come shifted by four bits), then the mask of the values held apart (X = 0
+// there), then padding that keeps the lanes' 16-byte reads of neighbouring blocks in distinct
+// banks.
+//
+// Held apart are NaN, infinities, and the largest values as long as fewer than four of the 32
+// (of those that are left) reach a 32nd of the largest: none among normal values, some in one of
+// 10000 blocks of h (a product of two), one or two in a block with an activation of a hundred times
+// its neighbours' size, and all where fewer than four are not 0 or 2^e would pass its range (below
+// 2^-99).
 // ---------------------------------------------------------------------------
-constexpr int FX_WORDS = 28;
+constexpr int FX_WORDS = 28, FX_SCALE = 24, FX_APART = 25;
 
-// v: this lane's elements 4j..4j+3 of a block, j = lane % 8; all 32 lanes call it
-PI_DEV void fix_block(const float4 v, uint32_t* blk, int j, bool store) {
-    float m = max_nan(max_nan(fabsf(v.x), fabsf(v.y)), max_nan(fabsf(v.z), fabsf(v.w)));
+// Which of a lane's four values of a block are held apart, and the largest magnitude of the block's
+// others. All 32 lanes call it, for one odd block among theirs: rare.
+__device__ __noinline__ uint2 hold_apart(float4 v) {
+    float e[4] = {v.x, v.y, v.z, v.w}, m = 0.0f;
+    uint32_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (!(fabsf(e[i]) < INFINITY)) {
+            mine |= 1u << i;
+            e[i] = 0.0f;
+        }
+        m = fmaxf(m, fabsf(e[i]));
+    }
+    while (true) {
+        int n = 0;
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const float lim = m * 0x1p-5f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) n += fabsf(e[i]) >= lim;
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+        const bool part = m > 0.0f && (n < 4 || m < 0x1p-99f);
+        if (!__any_sync(0xffffffffu, part)) return make_uint2(mine, __float_as_uint(m));
+        if (part) {
+            m = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (fabsf(e[i]) > 0.0f && fabsf(e[i]) >= lim) {
+                    mine |= 1u << i;
+                    e[i] = 0.0f;
+                }
+                m = fmaxf(m, fabsf(e[i]));
+            }
+        }
+    }
+}
+
+// v: this lane's elements 4j..4j+3 of a block, j = lane % 8; all 32 lanes call it. The lane's
+// values are stored at `apart` too where one of them is held apart (null: they are kept elsewhere).
+// Returns the block's mask.
+PI_DEV uint32_t fix_block(const float4 v, uint32_t* blk, int j, bool store, float* apart) {
+    const float own = max_nan(max_nan(fabsf(v.x), fabsf(v.y)), max_nan(fabsf(v.z), fabsf(v.w)));
+    float m = own, e[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const bool fin = m < INFINITY;
-    const int ex = fin && m > 0.0f ? min(21 - ilogbf(m), 120) : 0;
-    const float s = fin ? ldexpf(1.0f, ex) : 0.0f, e[4] = {v.x, v.y, v.z, v.w};
+    // a block is as most are where four of its lanes reach the limit
+    const uint32_t reach = __ballot_sync(0xffffffffu, own >= m * 0x1p-5f) >> (threadIdx.x & 24);
+    uint32_t mine = 0, all = 0;
+    if (__any_sync(0xffffffffu, !(m < INFINITY) || (m > 0.0f && (m < 0x1p-99f || __popc(reach & 255u) < 4)))) {
+        const uint2 r = hold_apart(v);
+        mine = r.x;
+        m = __uint_as_float(r.y);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if ((mine >> i) & 1) e[i] = 0.0f;
+        all = mine << (4 * j);
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) all |= __shfl_xor_sync(0xffffffffu, all, o);
+    }
+    const int ex = m > 0.0f ? 21 - ilogbf(m) : 0;
+    const float s = ldexpf(1.0f, ex);
     uint32_t even[3] = {0, 0, 0}, odd[3] = {0, 0, 0};  // two bytes of each term
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int X = fin ? __float2int_rn(e[i] * s) : 0;
+        const int X = __float2int_rn(e[i] * s);
         const int q3 = (int)(int8_t)X, X2 = (X - q3) >> 8, q2 = (int)(int8_t)X2, q1 = (X2 - q2) >> 8;
         uint32_t* to = i & 1 ? odd : even;
         to[0] |= (uint32_t)(q1 & 255) << (8 * (i >> 1));
         to[1] |= (uint32_t)(q2 & 255) << (8 * (i >> 1));
         to[2] |= (uint32_t)(q3 & 255) << (8 * (i >> 1));
     }
-    if (!store) return;
+    if (!store) return 0;
+    if (apart && mine) *reinterpret_cast<float4*>(apart) = v;
     uint16_t* h = reinterpret_cast<uint16_t*>(blk);
 #pragma unroll
     for (int t = 0; t < 3; ++t) {
         h[t * 16 + (j >> 1) * 4 + (j & 1)] = (uint16_t)even[t];
         h[t * 16 + (j >> 1) * 4 + 2 + (j & 1)] = (uint16_t)odd[t];
     }
-    if (j == 0) blk[24] = __float_as_uint(fin ? ldexpf(0.0625f, -ex) : __int_as_float(0x7fffffff));
+    if (j == 0) *reinterpret_cast<uint2*>(blk + FX_SCALE) = make_uint2(__float_as_uint(ldexpf(0.0625f, -ex)), all);
+    return all;
+}
+
+// Element i of a Q4_0 block of bytes at q, times the block's scale.
+PI_DEV float nib_value(const uint8_t* q, int i, __half d) {
+    return __half2float(d) * (float)(((__ldg(q + (i >> 1)) >> (4 * (i & 1))) & 15) - 8);
 }
 
 // nibbles of a word as 16 (n - 8) in int8: even elements, odd elements
@@ -102,6 +173,7 @@ struct FewLogitArgs {
     int T, d, E, R, norm;
     float *logits, *eps;  // [T][E + 1], eps: the bounds
     uint32_t *xfix, *bar;  // xfix [T][d / 32][FX_WORDS]: the (normed) inputs in fixed point
+    float* xap;            // [T][d]: those held apart, nothing elsewhere
 };
 
 __global__ __launch_bounds__(FL_T) void k_few_logits(const FewLogitArgs a) {
@@ -150,7 +222,8 @@ __global__ __launch_bounds__(FL_T) void k_few_logits(const FewLogitArgs a) {
         const bool in = o < nt * (d / 32);
         const int t = in ? o / (d / 32) : 0, b = in ? o - t * (d / 32) : 0, i = b * 32 + 4 * j;
         const float4 v = *reinterpret_cast<const float4*>(s_x + t * pitch + (i / S) * (S + 4) + (i & (S - 1)));
-        fix_block(v, a.xfix + ((int64_t)(t0 + t) * (d / 32) + b) * FX_WORDS, j, in);
+        fix_block(v, a.xfix + ((int64_t)(t0 + t) * (d / 32) + b) * FX_WORDS, j, in,
+                  a.xap + (int64_t)(t0 + t) * d + i);
     }
     for (int q = warp; q < nrow * nt; q += FL_W) {
         const int r = q / nt, t = q - r * nt, e = e0 + r;
@@ -193,6 +266,7 @@ __global__ __launch_bounds__(FL_T) void k_few_logits(const FewLogitArgs a) {
 // ---------------------------------------------------------------------------
 constexpr int FE_T = 512, FE_W = FE_T / 32;
 constexpr int FE_TB = 4;         // tokens at most that share a decoded weight
+constexpr int FE_SLOTS = 33;     // experts of a token and the shared one at most
 constexpr int FE_PART = 512;     // (column group, expert) sums of a CTA kept at a time
 constexpr int FE_MAXE = 513;     // experts and the shared one (a layer has 512 at most, a thread each)
 constexpr int FE_ITEMS = FE_MAXE + FEW_T / FE_TB;
@@ -202,6 +276,7 @@ struct FewExpertArgs {
     const __half *gd, *ud, *dd, *gsd, *usd, *dsd;    // their block scales
     const float* x;                                  // the layer's input
     const uint32_t* xfix;
+    const float* xap;
     const float *logits, *eps, *router, *bias;
     int T, d, f, E, k, has_shared, has_shgate, norm, residual;
     int group, n_groups;  // tokens whose inputs a CTA keeps for gate/up; such groups
@@ -271,16 +346,111 @@ PI_DEV void chunk_products(const RowChunk& k, const uint32_t* const (&xs)[TB], i
     }
 #pragma unroll
     for (int t = 0; t < TB; ++t) {
-        const float sx = __uint_as_float(xs[t][blk * FX_WORDS + 24]);
+        const float sx = __uint_as_float(xs[t][blk * FX_WORDS + FX_SCALE]);
 #pragma unroll
         for (int v = 0; v < 4; ++v)
             sum[v][t] = fmaf(__half2float(k.s[v]) * sx, fix_value(dot[v][t]), sum[v][t]);
     }
 }
 
+// Which inputs of a group's tokens are held apart: a bit for each block that has some, and where they
+// are few the list of them in order, each with its value in every token (0 where it is not held
+// apart). Outliers mostly stand at the same few places in every token.
+constexpr int AP_LIST = 64;
+struct ApartInputs {
+    uint32_t any, n;  // n > AP_LIST: too many for the list
+    uint32_t blk[FEW_T][4];
+    uint16_t at[AP_LIST];
+    float value[FEW_T][AP_LIST];
+};
+
+// The list, by the whole CTA; rare.
+template <int CPL>
+__device__ __noinline__ void list_apart(ApartInputs& s, const uint32_t* s_x, const float* xap, int nt) {
+    constexpr int nb = 32 * CPL;
+    const int tid = threadIdx.x;
+    if (tid < 32) {
+        int n = 0;
+        for (int c = 0; c < CPL; ++c) {
+            uint32_t m = 0;  // of block tid + 32 c in any token
+            for (int t = 0; t < nt; ++t) m |= s_x[(t * nb + tid + 32 * c) * FX_WORDS + FX_APART];
+            int upto = __popc(m);
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (tid >= o) upto += v;
+            }
+            for (int i = n + upto - __popc(m); m; m &= m - 1, ++i)
+                if (i < AP_LIST) s.at[i] = (uint16_t)((tid + 32 * c) * 32 + __ffs(m) - 1);
+            n += __shfl_sync(0xffffffffu, upto, 31);
+        }
+        if (tid == 0) s.n = n;
+    }
+    __syncthreads();
+    if (s.n <= AP_LIST)
+        for (int i = tid; i < nt * AP_LIST; i += FE_T) {
+            const int t = i / AP_LIST, q = i % AP_LIST;
+            float v = 0.0f;
+            if (q < s.n && (s_x[(t * nb + (s.at[q] >> 5)) * FX_WORDS + FX_APART] >> (s.at[q] & 31)) & 1)
+                v = xap[t * nb * 32 + s.at[q]];
+            s.value[t][q] = v;
+        }
+    __syncthreads();
+}
+
+// c[t] += this lane's part of what the values held apart add to row-vector lane / 8 of an item's unit
+// (rows row, row + 1 of expert e) for its tokens, numbered in the bytes of toks within the CTA's
+// group: every eighth of the list, or of the elements of the blocks that have some. The weights,
+// read a moment ago, come from L2. A function of its own: it is rare, and the loop around it has
+// no registers to spare.
+template <int CPL>
+__device__ __noinline__ float4 apart_products(const FewExpertArgs& a, const ApartInputs& s, const uint32_t* s_x, int t0,
+                                              uint32_t toks, int e, int row, float4 c, int lane) {
+    constexpr int d = 1024 * CPL, nb = d / 32;
+    const bool up = lane & 8, sh = e == a.E;
+    const int64_t r = (sh ? 0 : (int64_t)e * a.f) + row + (lane >> 4);
+    const uint8_t* w = (up ? (sh ? a.us : a.u) : (sh ? a.gs : a.g)) + r * (d / 2);
+    const __half* sc = (up ? (sh ? a.usd : a.ud) : (sh ? a.gsd : a.gd)) + r * nb;
+    const int tok[FE_TB] = {(int)(toks & 255), (int)(toks >> 8 & 255), (int)(toks >> 16 & 255), (int)(toks >> 24)};
+    float sum[FE_TB] = {c.x, c.y, c.z, c.w};
+    if (s.n <= AP_LIST) {
+#pragma unroll 2
+        for (int q = lane & 7; q < s.n; q += 8) {
+            const int at = s.at[q];
+            const float v = nib_value(w + (at >> 5) * 16, at & 31, sc[at >> 5]);
+#pragma unroll
+            for (int t = 0; t < FE_TB; ++t) sum[t] = fmaf(v, s.value[tok[t]][q], sum[t]);
+        }
+        return make_float4(sum[0], sum[1], sum[2], sum[3]);
+    }
+    for (int q = 0; q < CPL; ++q) {
+        uint32_t blks = 0;
+#pragma unroll
+        for (int t = 0; t < FE_TB; ++t) blks |= s.blk[tok[t]][q];
+        for (; blks; blks &= blks - 1) {
+            const int b = 32 * q + __ffs(blks) - 1;
+            uint32_t mask[FE_TB], any = 0;
+#pragma unroll
+            for (int t = 0; t < FE_TB; ++t) {
+                mask[t] = s_x[(tok[t] * nb + b) * FX_WORDS + FX_APART] >> (lane & 7);
+                any |= mask[t];
+            }
+            for (int i = 0; i < 32; i += 8) {
+                if (!((any >> i) & 1)) continue;
+                const float v = nib_value(w + b * 16, i + (lane & 7), sc[b]);
+#pragma unroll
+                for (int t = 0; t < FE_TB; ++t)
+                    if ((mask[t] >> i) & 1)
+                        sum[t] = fmaf(v, a.xap[(int64_t)(t0 + tok[t]) * d + b * 32 + i + (lane & 7)], sum[t]);
+            }
+        }
+    }
+    return make_float4(sum[0], sum[1], sum[2], sum[3]);
+}
+
 // All chunks of a unit for TB tokens, the unit's first chunk being in `k`; leaves there the first
 // chunk of the next unit (at `next`), which is on its way while the last one is worked on.
-// sum[t]: lanes 0-7 the first row's gate, 8-15 its up, 16-23 the second row's gate, 24-31 its up.
+// out[t]: eight parts of each row's sum, in lanes 0-7 those of the first row's gate, 8-15 of its up, 16-23
+// of the second row's gate, 24-31 of its up.
 template <int CPL, int TB>
 PI_DEV void gateup_rows(RowChunk& k, const RowPtrs& at, const RowPtrs& next, const uint32_t* const (&xs)[TB],
                         int lane, float* out) {
@@ -306,11 +476,7 @@ PI_DEV void gateup_rows(RowChunk& k, const RowPtrs& at, const RowPtrs& next, con
         float a = hi ? sum[2][t] : sum[0][t], b = hi ? sum[3][t] : sum[1][t];
         a += __shfl_xor_sync(0xffffffffu, hi ? sum[0][t] : sum[2][t], 16);
         b += __shfl_xor_sync(0xffffffffu, hi ? sum[1][t] : sum[3][t], 16);
-        float c = mid ? b : a;
-        c += __shfl_xor_sync(0xffffffffu, mid ? a : b, 8);
-#pragma unroll
-        for (int o = 4; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
-        out[t] = c;
+        out[t] = (mid ? b : a) + __shfl_xor_sync(0xffffffffu, mid ? a : b, 8);
     }
 }
 
@@ -351,13 +517,38 @@ struct DownRows {
                     dot[p] = dp4a((int)n[3], x.w, dot[p]);
                 }
             }
-            sum = fmaf(__half2float(s[b]) * __uint_as_float(hp[b * FX_WORDS + 24]), fix_value(dot), sum);
+            sum = fmaf(__half2float(s[b]) * __uint_as_float(hp[b * FX_WORDS + FX_SCALE]), fix_value(dot), sum);
         }
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
         return sum;
     }
 };
+// Adds what the values of h held apart give to the sums of a pass, part[unit][expert][column] of n units of
+// eight columns from col0 on: blks[expert] has a bit for each block that has some, s_h is the
+// fixed-point h and h its f32 values. By the whole CTA; rare.
+template <int BPQ>
+__device__ __noinline__ void apart_down(const FewExpertArgs& a, const int* idx, const uint32_t* blks, const uint32_t* s_h,
+                                        const float* h, int n, int col0, float* part) {
+    constexpr int f = 128 * BPQ, hp = 4 * BPQ * FX_WORDS + (BPQ == 1 ? 0 : 16);
+    const int slots = a.k + a.has_shared;
+    for (int i = threadIdx.x; i < n * slots * 8; i += FE_T) {
+        const int v = i / (8 * slots), j = (i >> 3) - v * slots;
+        const bool sh = j == a.k;
+        const int64_t row = (sh ? 0 : (int64_t)idx[j] * a.d) + col0 + 8 * v;  // eight rows are tiled together
+        const uint8_t* D = (sh ? a.dns : a.dn) + row * (f / 2);
+        const __half* DD = (sh ? a.dsd : a.dd) + row * (f / 32);
+        float s = 0.0f;
+        for (uint32_t m = blks[j]; m; m &= m - 1) {
+            const int q = (__ffs(m) - 1) / BPQ, b = (__ffs(m) - 1) % BPQ, lane = 4 * (i & 7) + q;
+            for (uint32_t e = s_h[j * hp + q * h_quarter(BPQ) + b * FX_WORDS + FX_APART]; e; e &= e - 1)
+                s = fmaf(nib_value(D + (b * 32 + lane) * 16, __ffs(e) - 1, DD[lane * BPQ + b]),
+                         __ldcg(h + j * f + (q * BPQ + b) * 32 + __ffs(e) - 1), s);
+        }
+        part[i] += s;
+    }
+    __syncthreads();
+}
 
 // Barrier of a cooperatively launched grid, used once: *bar counts up from 0. The wait is
 // bounded (2^24 polls, the later ones 32 ns apart: about half a second); when it runs out
@@ -503,7 +694,7 @@ struct FewRouting {  // in shared memory: [T][k], [T][k], [T]
 // before the barrier, each next one's on their way while one is worked on.
 template <int BPQ>
 PI_DEV void down_phase(const FewExpertArgs& a, const int d, const FewRouting& r, uint32_t* s_h, float* s_part,
-                       int* s_ok) {
+                       uint32_t (*s_apart)[FE_SLOTS + 1], int* s_ok) {
     constexpr int f = 128 * BPQ, hp = 4 * BPQ * FX_WORDS + (BPQ == 1 ? 0 : 16);  // hp: words of an expert's h
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int T = a.T, k = a.k, slots = k + a.has_shared, per_tok = d / 8;
@@ -524,24 +715,34 @@ PI_DEV void down_phase(const FewExpertArgs& a, const int d, const FewRouting& r,
     auto pass = [&](int u) {  // units of one token that are summed together, a thread for each column
         return min(min(FE_PART / slots, FE_T / 8), min(ue, (u / per_tok + 1) * per_tok) - u);
     };
-    if (ub < ue && warp < pass(ub) * slots) load(cur, ub / per_tok, ub % per_tok * 8, v0, j0);
-    float residual = a.residual && ub < ue && tid < pass(ub) * 8 ? a.x[(int64_t)ub * 8 + tid] : 0.0f;
+    float residual = 0.0f;
+    auto begin = [&](int u) {  // a warp's first weights of the pass from unit u on
+        const int t = u / per_tok, n = pass(u);
+        if (warp < n * slots) load(cur, t, (u - t * per_tok) * 8, v0, j0);
+        if (a.residual && tid < n * 8) residual = a.x[(int64_t)u * 8 + tid];
+    };
+    if (ub < ue) begin(ub);
+    if (tid <= FE_SLOTS) s_apart[0][tid] = 0;
     if (!grid_barrier(a.bar, a.err, s_ok)) return;
-    for (int u = ub, tok = -1; u < ue;) {
+    for (int u = ub, tok = -1, turn = 1; u < ue;) {
         const int t = u / per_tok, n = pass(u), col0 = (u - t * per_tok) * 8;
         if (t != tok) {
             const float* ht = a.h + (int64_t)t * slots * f;
+            turn ^= 1;  // this token's masks; the next one's are cleared meanwhile
             for (int i0 = 0; i0 < slots * (f / 4); i0 += FE_T) {  // whole warps: eight lanes make a block
                 const int i = min(i0 + tid, slots * (f / 4) - 1), j = i / (f / 4), b = (i & (f / 4 - 1)) >> 3;
-                fix_block(__ldcg(reinterpret_cast<const float4*>(ht) + i),
-                          s_h + j * hp + (b / BPQ) * h_quarter(BPQ) + (b % BPQ) * FX_WORDS, i & 7,
-                          i0 + tid < slots * (f / 4));
+                const uint32_t apart = fix_block(__ldcg(reinterpret_cast<const float4*>(ht) + i),
+                                                 s_h + j * hp + (b / BPQ) * h_quarter(BPQ) + (b % BPQ) * FX_WORDS,
+                                                 i & 7, i0 + tid < slots * (f / 4), nullptr);
+                if (apart && (i & 7) == 0) {
+                    atomicOr(&s_apart[turn][j], 1u << b);
+                    s_apart[turn][FE_SLOTS] = 1;
+                }
             }
+            if (tid <= FE_SLOTS) s_apart[turn ^ 1][tid] = 0;
             tok = t;
             __syncthreads();
         }
-        if (u != ub && warp < n * slots) load(cur, t, col0, v0, j0);
-        if (u != ub && a.residual && tid < n * 8) residual = a.x[(int64_t)u * 8 + tid];
         for (int i = warp, v = v0, j = j0; i < n * slots; i += FE_W) {
             const int now = j;
             v += dv;
@@ -556,6 +757,8 @@ PI_DEV void down_phase(const FewExpertArgs& a, const int d, const FewRouting& r,
             cur = nxt;
         }
         __syncthreads();
+        if (s_apart[turn][FE_SLOTS])
+            apart_down<BPQ>(a, r.idx + t * k, s_apart[turn], s_h, a.h + (int64_t)t * slots * f, n, col0, s_part);
         if (tid < n * 8) {  // model/mod.rs:1525-1534, :1627-1633
             const float* p = s_part + (tid >> 3) * slots * 8 + (tid & 7);
             float acc = 0.0f;
@@ -565,18 +768,21 @@ PI_DEV void down_phase(const FewExpertArgs& a, const int d, const FewRouting& r,
         }
         __syncthreads();
         u += n;
+        cur = DownRows<BPQ>();  // nothing of it is kept over the rare call above
+        if (u < ue) begin(u);
     }
 }
 
-template <int CPL, int NPL>
-__global__ __launch_bounds__(FE_T, 1) void k_few_experts(const FewExpertArgs a) {
+template <int CPL, int NPL, int BPQ>
+__global__ __launch_bounds__(FE_T, 1) void k_few_experts(const __grid_constant__ FewExpertArgs a) {
     extern __shared__ __align__(16) uint32_t s_dyn[];  // gate/up: inputs of the group's tokens; down: h
     __shared__ int s_idx[FEW_T * 32], s_use[FE_ITEMS], s_mask[FE_T], s_item[FE_ITEMS], s_count[FE_W], s_nuse, s_ok;
-    __shared__ uint32_t s_open;
+    __shared__ ApartInputs s_apart;
+    __shared__ uint32_t s_open, s_hblk[2][FE_SLOTS + 1];
     __shared__ float s_gate[FEW_T * 32], s_share[FEW_T], s_inv, s_part[FE_PART * 8];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    constexpr int d = 1024 * CPL, nb = d / 32;
-    const int T = a.T, f = a.f, E = a.E, k = a.k, slots = k + a.has_shared;
+    constexpr int d = 1024 * CPL, nb = d / 32, f = 128 * BPQ;
+    const int T = a.T, E = a.E, k = a.k, slots = k + a.has_shared;
     const int grp = blockIdx.x % a.n_groups, t0 = grp * a.group, nt = min(a.group, T - t0);
     const int cta = blockIdx.x / a.n_groups, n_cta = (gridDim.x - grp + a.n_groups - 1) / a.n_groups;
 
@@ -588,7 +794,7 @@ __global__ __launch_bounds__(FE_T, 1) void k_few_experts(const FewExpertArgs a) 
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
     // routing of every token (a warp each), in every CTA
-    if (tid == 0) s_open = 0;
+    if (tid == 0) s_open = s_apart.any = 0;
     s_mask[tid] = 0;
     __syncthreads();
     if (warp < T &&
@@ -610,7 +816,16 @@ __global__ __launch_bounds__(FE_T, 1) void k_few_experts(const FewExpertArgs a) 
     // weights. The shared expert's come first, then those of several tokens, so that the
     // heaviest are spread evenly over the warps. Thread e counts the items of expert e.
     for (int i = tid; i < nt * k; i += FE_T) atomicOr(&s_mask[s_idx[t0 * k + i]], 1 << (i / k));
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
+    if (warp < nt)  // which blocks of its inputs have values held apart
+#pragma unroll
+        for (int c = 0; c < CPL; ++c) {
+            const uint32_t b =
+                __ballot_sync(0xffffffffu, s_dyn[(warp * nb + lane + 32 * c) * FX_WORDS + FX_APART] != 0);
+            if (lane == 0) s_apart.blk[warp][c] = b;
+            if (lane == 0 && b) s_apart.any = 1;
+        }
     {
         const int n_sh = a.has_shared ? (nt + FE_TB - 1) / FE_TB : 0;
         int m = tid < E ? s_mask[tid] : 0;
@@ -648,11 +863,11 @@ __global__ __launch_bounds__(FE_T, 1) void k_few_experts(const FewExpertArgs a) 
         }
         if (tid == 0) s_nuse = n_sh + heavy + (total >> 16);
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
 
     // gate, up and SwiGLU: a warp takes two rows of an expert for the tokens of an item
-    const int half_f = f / 2, lf = 31 - __clz(half_f), n_unit = s_nuse * half_f, stride = n_cta * FE_W;
+    constexpr int half_f = f / 2;
+    const int lf = 31 - __clz(half_f), n_unit = s_nuse * half_f, stride = n_cta * FE_W;
     auto rows = [&](int unit) {
         const int e = s_use[unit >> lf], r = 2 * (unit & (half_f - 1));
         if (e == E)
@@ -660,58 +875,75 @@ __global__ __launch_bounds__(FE_T, 1) void k_few_experts(const FewExpertArgs a) 
         const int64_t q = (int64_t)(e * f + r);  // E f < 2^20
         return RowPtrs{a.g + q * (d / 2), a.u + q * (d / 2), a.gd + q * nb, a.ud + q * nb};
     };
-    RowChunk chunk;
-    RowPtrs at = {}, next = {};
-    const int first = cta * FE_W + warp;
-    if (first < n_unit) {
-        at = rows(first);
-        chunk.load(at, nb, lane);
-    }
-    for (int unit = first; unit < n_unit; unit += stride) {
-        const int item = unit >> lf, e = s_use[item], row = 2 * (unit & (half_f - 1));
-        uint32_t mask = s_item[item];
-        next = unit + stride < n_unit ? rows(unit + stride) : at;  // the last one reads its own first chunk again
-        int tok[FE_TB], n = 0;
-        const uint32_t* xs[FE_TB];
+    auto gate_up = [&](auto any) {
+        constexpr bool APART = decltype(any)::value;
+        RowChunk chunk;
+        RowPtrs at = {}, next = {};
+        const int first = cta * FE_W + warp;
+        if (first < n_unit) {
+            at = rows(first);
+            chunk.load(at, nb, lane);
+        }
+        for (int unit = first; unit < n_unit; unit += stride) {
+            const int item = unit >> lf, e = s_use[item], row = 2 * (unit & (half_f - 1));
+            uint32_t mask = s_item[item];
+            next = unit + stride < n_unit ? rows(unit + stride) : at;  // the last one reads its own first chunk again
+            int tok[FE_TB], n = 0;
+            const uint32_t* xs[FE_TB];
 #pragma unroll
-        for (int i = 0; i < FE_TB; ++i) {  // an item that is not full repeats its last token
-            if (mask) {
-                tok[i] = __ffs(mask) - 1;
-                mask &= mask - 1;
-                ++n;
-            } else {
-                tok[i] = tok[i > 0 ? i - 1 : 0];
+            for (int i = 0; i < FE_TB; ++i) {  // an item that is not full repeats its last token
+                if (mask) {
+                    tok[i] = __ffs(mask) - 1;
+                    mask &= mask - 1;
+                    ++n;
+                } else {
+                    tok[i] = tok[i > 0 ? i - 1 : 0];
+                }
+                xs[i] = s_dyn + tok[i] * nb * FX_WORDS;
             }
-            xs[i] = s_dyn + tok[i] * nb * FX_WORDS;
-        }
-        float sum[FE_TB];
-        if (n == 1) {
-            const uint32_t* const x1[1] = {xs[0]};
-            gateup_rows<CPL, 1>(chunk, at, next, x1, lane, sum);
-        } else if (n == 2) {
-            const uint32_t* const x2[2] = {xs[0], xs[1]};
-            gateup_rows<CPL, 2>(chunk, at, next, x2, lane, sum);
-        } else {
-            gateup_rows<CPL, FE_TB>(chunk, at, next, xs, lane, sum);
-        }
+            float sum[FE_TB] = {};
+            if (n == 1) {
+                const uint32_t* const x1[1] = {xs[0]};
+                gateup_rows<CPL, 1>(chunk, at, next, x1, lane, sum);
+            } else if (n == 2) {
+                const uint32_t* const x2[2] = {xs[0], xs[1]};
+                gateup_rows<CPL, 2>(chunk, at, next, x2, lane, sum);
+            } else {
+                gateup_rows<CPL, FE_TB>(chunk, at, next, xs, lane, sum);
+            }
+            if constexpr (APART) {
+                const float4 c = apart_products<CPL>(a, s_apart, s_dyn, t0, tok[0] | tok[1] << 8 | tok[2] << 16 | tok[3] << 24,
+                                                     e, row, make_float4(sum[0], sum[1], sum[2], sum[3]), lane);
+                sum[0] = c.x;
+                sum[1] = c.y;
+                sum[2] = c.z;
+                sum[3] = c.w;
+            }
 #pragma unroll
-        for (int i = 0; i < FE_TB; ++i) {
-            if (i >= n) break;
-            const int t = t0 + tok[i];
-            int j = k;
-            if (e != E) j = __ffs(__ballot_sync(0xffffffffu, lane < k && s_idx[t * k + lane] == e)) - 1;
-            const float g = sum[i], u = __shfl_down_sync(0xffffffffu, g, 8);
-            if ((lane & 15) == 0) a.h[((int64_t)t * slots + j) * f + row + (lane >> 4)] = g / (1.0f + expf(-g)) * u;
+            for (int i = 0; i < FE_TB; ++i) {
+                if (i >= n) break;
+                const int t = t0 + tok[i];
+                int j = k;
+                if (e != E) j = __ffs(__ballot_sync(0xffffffffu, lane < k && s_idx[t * k + lane] == e)) - 1;
+                float g = sum[i];
+#pragma unroll
+                for (int o = 4; o > 0; o >>= 1) g += __shfl_xor_sync(0xffffffffu, g, o);
+                const float u = __shfl_down_sync(0xffffffffu, g, 8);
+                if ((lane & 15) == 0) a.h[((int64_t)t * slots + j) * f + row + (lane >> 4)] = g / (1.0f + expf(-g)) * u;
+            }
+            at = next;
         }
-        at = next;
+    };
+    // two loops: the call takes registers from the one that has it (16 tokens, 256 experts: 78 us, 80 with one).
+    // Four outliers in every token make 78 us 94, a single token's 19.5 us 23.3.
+    if (!s_apart.any) {
+        gate_up(std::false_type());
+    } else {
+        list_apart<CPL>(s_apart, s_dyn, a.xap + (int64_t)t0 * d, nt);
+        gate_up(std::true_type());
     }
     const FewRouting routing{s_idx, s_gate, s_share};
-    switch (f / 128) {
-        case 1: down_phase<1>(a, d, routing, s_dyn, s_part, &s_ok); break;
-        case 2: down_phase<2>(a, d, routing, s_dyn, s_part, &s_ok); break;
-        case 4: down_phase<4>(a, d, routing, s_dyn, s_part, &s_ok); break;
-        default: down_phase<8>(a, d, routing, s_dyn, s_part, &s_ok); break;
-    }
+    down_phase<BPQ>(a, d, routing, s_dyn, s_part, s_hblk, &s_ok);
 }
 
 // ---------------------------------------------------------------------------
@@ -722,6 +954,7 @@ constexpr size_t FEW_X_BYTES = 180 * 1024;  // inputs of the tokens a CTA keeps 
 struct FewBufs {
     float *logits, *eps, *h;
     uint32_t *xfix, *bar;
+    float* xap;
     size_t bytes;
 };
 FewBufs few_carve(const pi_moe_layer* L, int64_t T, char* base) {
@@ -731,16 +964,17 @@ FewBufs few_carve(const pi_moe_layer* L, int64_t T, char* base) {
     o.logits = b.take<float>(T * (L->E + 1));
     o.eps = b.take<float>(T * (L->E + 1));
     o.xfix = b.take<uint32_t>(T * (L->d / 32) * FX_WORDS);
+    o.xap = b.take<float>(T * L->d);
     o.h = b.take<float>(T * (L->k + (L->has_shared ? 1 : 0)) * L->f);
     o.bytes = b.off + 256;
     return o;
 }
 
-template <int CPL, int NPL>
+template <int CPL, int NPL, int BPQ>
 cudaError_t launch_experts(const FewExpertArgs& a, int sms, cudaStream_t st) {
     const size_t x = (size_t)a.group * (a.d / 32) * FX_WORDS * 4;
     const size_t h = (size_t)(a.k + a.has_shared) * (a.f / 32 * FX_WORDS + 16) * 4, smem = std::max(x, h);
-    auto kern = k_few_experts<CPL, NPL>;
+    auto kern = k_few_experts<CPL, NPL, BPQ>;
     // the limit is always raised: beside the kernel's 26 KB of static shared memory the default
     // of 48 KB would not hold what pi_smem_attr lets pass as small
     pi_smem_attr((const void*)kern, std::max<size_t>(smem, 64 * 1024));
@@ -755,6 +989,16 @@ cudaError_t launch_experts(const FewExpertArgs& a, int sms, cudaStream_t st) {
     cfg.attrs = at;
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kern, a);
+}
+
+template <int CPL, int NPL>
+cudaError_t launch_width(const FewExpertArgs& a, int sms, cudaStream_t st) {
+    switch (a.f) {
+        case 128: return launch_experts<CPL, NPL, 1>(a, sms, st);
+        case 256: return launch_experts<CPL, NPL, 2>(a, sms, st);
+        case 512: return launch_experts<CPL, NPL, 4>(a, sms, st);
+        default: return launch_experts<CPL, NPL, 8>(a, sms, st);
+    }
 }
 
 int few_forward(pi_ctx* ctx, const pi_moe_layer* L, const float* x, int64_t T, float* out, int flags, void* workspace,
@@ -787,7 +1031,8 @@ int few_forward(pi_ctx* ctx, const pi_moe_layer* L, const float* x, int64_t T, f
         const int R = (int)std::min<int64_t>(fit, std::max<int64_t>(2, ((E + 1) * groups + sms - 1) / sms));
         const size_t smem = row * (FL_GROUP + R);
         pi_smem_attr((const void*)k_few_logits, smem);
-        const FewLogitArgs a{x, L->router, L->bias, (int)T, d, E, R, norm ? 1 : 0, B.logits, B.eps, B.xfix, B.bar};
+        const FewLogitArgs a{x, L->router, L->bias, (int)T, d, E, R, norm ? 1 : 0, B.logits, B.eps, B.xfix, B.bar,
+                             B.xap};
         pi_pdl_launch(k_few_logits, dim3((unsigned)((E + R) / R), (unsigned)groups), dim3(FL_T), smem, st, a);
         if (int rc = pi_cuda_check(ctx, cudaGetLastError(), "moe fused logits")) return rc;
     }
@@ -810,6 +1055,7 @@ int few_forward(pi_ctx* ctx, const pi_moe_layer* L, const float* x, int64_t T, f
     }
     a.x = x;
     a.xfix = B.xfix;
+    a.xap = B.xap;
     a.logits = B.logits;
     a.eps = B.eps;
     a.router = L->router;
@@ -833,9 +1079,9 @@ int few_forward(pi_ctx* ctx, const pi_moe_layer* L, const float* x, int64_t T, f
     const bool wide = E > 256;
     cudaError_t e;
     switch (d / 1024) {
-        case 1: e = wide ? launch_experts<1, 16>(a, sms, st) : launch_experts<1, 8>(a, sms, st); break;
-        case 2: e = wide ? launch_experts<2, 16>(a, sms, st) : launch_experts<2, 8>(a, sms, st); break;
-        default: e = wide ? launch_experts<4, 16>(a, sms, st) : launch_experts<4, 8>(a, sms, st); break;
+        case 1: e = wide ? launch_width<1, 16>(a, sms, st) : launch_width<1, 8>(a, sms, st); break;
+        case 2: e = wide ? launch_width<2, 16>(a, sms, st) : launch_width<2, 8>(a, sms, st); break;
+        default: e = wide ? launch_width<4, 16>(a, sms, st) : launch_width<4, 8>(a, sms, st); break;
     }
     return pi_cuda_check(ctx, e, "moe fused experts");
 }

@@ -99,7 +99,8 @@ class MoeLayer:
 
         path: "auto" (tensor-core GEMM for prefill-sized Q4_0 batches, else GEMV),
         "gemv" or "gemm" to force one; "fused": at most 16 tokens of a Q4_0 layer in two
-        kernels (``pi_moe_forward_fused``; the routing of ``route``, sums in another
+        kernels (``pi_moe_forward_fused``; the experts of ``route``, inputs held in f32
+        or within 2^-17 of the fourth largest of their block of 32, sums in another
         order than "gemv"). fast: the Q8_0 prefill GEMM adds each block
         term with a fused multiply-add (PI_FWD_FAST_SUM; within the parity tolerance,
         not bit-identical).
