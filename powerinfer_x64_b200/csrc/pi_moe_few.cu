@@ -10,8 +10,9 @@
 // (quant/mod.rs:921-935), about 4.2 dependent cycles an input: 5.5 us of a token's 29 at
 // n_embd 2048. Here a logit is summed in 32 segments side by side with a bound of how far
 // the sequential sum can be from it, and a choice that the bounds leave open (0.4% of
-// tokens for normal inputs, and exact ties) is made again from sequential logits and the
-// reference's own softmax and top-k (pi_topk.cuh).
+// tokens for normal inputs, and exact ties) is made again from sequential logits, which the
+// whole grid makes at the price of one more barrier, and the reference's own softmax and top-k
+// (pi_topk.cuh).
 //
 // Expert products: the reference dequantises Q4_0 rows and sums f32 products (quant/mod.rs:
 // 958-969). Here 32 inputs that share a weight scale become fixed-point numbers of 22 bits
@@ -196,7 +197,7 @@ __global__ __launch_bounds__(FL_T) void k_few_logits(const FewLogitArgs a) {
     fetch(s_w, a.router + (int64_t)e0 * d, nrow);  // constant weights: before the wait
     pdl_wait();
     fetch(s_x, a.x + (int64_t)t0 * d, nt);
-    if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) *a.bar = 0;  // of the next kernel
+    if (blockIdx.x == 0 && blockIdx.y == 0 && tid < 2) a.bar[tid] = 0;  // of the next kernel
     asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
     __syncthreads();
     if (a.norm) {
@@ -280,6 +281,7 @@ struct FewExpertArgs {
     const float *logits, *eps, *router, *bias;
     int T, d, f, E, k, has_shared, has_shgate, norm, residual;
     int group, n_groups;  // tokens whose inputs a CTA keeps for gate/up; such groups
+    float *exact;         // [T][E + 1], of tokens that the bounds leave open
     float *h, *out;       // h [T][k + shared][f]
     uint32_t *bar, *err;
 };
@@ -550,7 +552,7 @@ __device__ __noinline__ void apart_down(const FewExpertArgs& a, const int* idx, 
     __syncthreads();
 }
 
-// Barrier of a cooperatively launched grid, used once: *bar counts up from 0. The wait is
+// Barrier of a cooperatively launched grid, each used once: *bar counts up from 0. The wait is
 // bounded (2^24 polls, the later ones 32 ns apart: about half a second); when it runs out
 // the kernel records PI_DEVERR_TIMEOUT and the CTA returns.
 PI_DEV bool grid_barrier(uint32_t* bar, uint32_t* err, int* s_ok) {
@@ -646,42 +648,92 @@ PI_DEV bool topk_certain(const float* logits, const float* eps, int E, int k, in
     return true;
 }
 
-// The reference's logits of one token, by the whole CTA: its norm (four sequential sums of
-// squares, simd.rs:116-137) and one sequential chain a thread. Only for tokens that
-// topk_certain leaves open.
-PI_DEV void exact_logits(const float* x, const float* router, const float* bias, int d, int E, int norm,
-                         float* out, float* s_inv) {
-    const int tid = threadIdx.x;
-    if (norm && tid < 32) {
-        float acc = 0.0f;
-        if (tid < 4)
+// The reference's logits of the tokens in `open`, to a.exact [T][E + 1]: norms (four sequential sums of
+// squares, simd.rs:116-137) by a warp a token in every CTA, then sequential chains, a thread for each
+// of the CTA's rows and open tokens; the CTAs of the grid share the rows. Both go through
+// shared memory (s: FE_PART * 8 floats), in coalesced pieces of which the next is on its way. Only
+// for tokens that topk_certain leaves open: 18 us for three of n_embd 2048 and 256 experts, 28 for
+// fifteen, 7 of them the norms (each CTA making all chains for itself, token by token: 90 us a token).
+constexpr int EX_COLS = 128, EX_PITCH = EX_COLS + 4;
+__device__ __noinline__ void exact_logits(const FewExpertArgs& a, uint32_t open, float* s) {
+    __shared__ int s_tok[FEW_T];
+    __shared__ float s_inv[FEW_T];
+    constexpr int ROWS = FE_PART * 8 / EX_PITCH, PER = (ROWS * EX_COLS / 4 + FE_T - 1) / FE_T;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n = __popc(open), d = a.d;
+    if (tid < 32 && (open >> tid) & 1) s_tok[__popc(open & ((1u << tid) - 1u))] = tid;
+    __syncthreads();
+    if (warp < n) {
+        float inv = 1.0f;
+        if (a.norm) {
+            const float* x = a.x + (int64_t)s_tok[warp] * d + lane * 4;
+            float *strip = s + warp * 256, acc = 0.0f;
+            float4 v = *reinterpret_cast<const float4*>(x), w = *reinterpret_cast<const float4*>(x + 128);
+            for (int c = 0; c < d; c += 256) {
+                *reinterpret_cast<float4*>(strip + lane * 4) = v;
+                *reinterpret_cast<float4*>(strip + 128 + lane * 4) = w;
+                __syncwarp();
+                if (c + 256 < d) {
+                    v = *reinterpret_cast<const float4*>(x + c + 256);
+                    w = *reinterpret_cast<const float4*>(x + c + 384);
+                }
+                if (lane < 4)
 #pragma unroll 16
-            for (int j = tid; j < d; j += 4) acc = fadd(acc, fmul(x[j], x[j]));
-        const float a1 = __shfl_sync(0xffffffffu, acc, 1), a2 = __shfl_sync(0xffffffffu, acc, 2),
-                    a3 = __shfl_sync(0xffffffffu, acc, 3);
-        if (tid == 0) {
-            const float ss = fadd(fadd(acc, a1), fadd(a2, a3));
-            *s_inv = fdiv(1.0f, __fsqrt_rn(fadd(fdiv(ss, (float)d), 1e-6f)));
+                    for (int j = lane; j < 256; j += 4) acc = fadd(acc, fmul(strip[j], strip[j]));
+                __syncwarp();
+            }
+            const float a1 = __shfl_sync(0xffffffffu, acc, 1), a2 = __shfl_sync(0xffffffffu, acc, 2),
+                        a3 = __shfl_sync(0xffffffffu, acc, 3);
+            inv = fdiv(1.0f, __fsqrt_rn(fadd(fdiv(fadd(fadd(acc, a1), fadd(a2, a3)), (float)d), 1e-6f)));
         }
+        if (lane == 0) s_inv[warp] = inv;
     }
     __syncthreads();
-    const float inv = norm ? *s_inv : 1.0f;
-    for (int e = tid; e <= E; e += FE_T) {
-        const float* w = router + (int64_t)e * d;
+    const int rows = a.E + 1, end = (int)((int64_t)rows * (blockIdx.x + 1) / gridDim.x);
+    for (int e0 = (int)((int64_t)rows * blockIdx.x / gridDim.x); e0 < end; e0 += ROWS - n) {
+        // a piece: columns of nr router rows, then of the n tokens
+        const int nr = min(ROWS - n, end - e0), r = tid / n, i = tid - r * n;
+        float4 v[PER];
+        auto fetch = [&](int c) {
+#pragma unroll
+            for (int q = 0; q < PER; ++q) {
+                const int at = tid + q * FE_T, row = at / (EX_COLS / 4), col = c + at % (EX_COLS / 4) * 4;
+                if (row < nr) v[q] = __ldg(reinterpret_cast<const float4*>(a.router + (int64_t)(e0 + row) * d + col));
+                else if (row < nr + n)
+                    v[q] = *reinterpret_cast<const float4*>(a.x + (int64_t)s_tok[row - nr] * d + col);
+            }
+        };
+        fetch(0);
         float acc = 0.0f;
+        for (int c = 0; c < d; c += EX_COLS) {
+#pragma unroll
+            for (int q = 0; q < PER; ++q) {
+                const int at = tid + q * FE_T, row = at / (EX_COLS / 4), col = at % (EX_COLS / 4) * 4;
+                if (row >= nr + n) continue;
+                float4 u = v[q];
+                if (a.norm && row >= nr) {
+                    const float inv = s_inv[row - nr];
+                    u = make_float4(fmul(u.x, inv), fmul(u.y, inv), fmul(u.z, inv), fmul(u.w, inv));
+                }
+                *reinterpret_cast<float4*>(s + row * EX_PITCH + col) = u;
+            }
+            __syncthreads();
+            if (c + EX_COLS < d) fetch(c + EX_COLS);
+            if (r < nr) {
+                const float *w = s + r * EX_PITCH, *x = s + (nr + i) * EX_PITCH;
 #pragma unroll 8
-        for (int i = 0; i < d; i += 4) {
-            const float4 a = __ldg(reinterpret_cast<const float4*>(w + i));
-            float4 v = *reinterpret_cast<const float4*>(x + i);
-            if (norm) v = make_float4(fmul(v.x, inv), fmul(v.y, inv), fmul(v.z, inv), fmul(v.w, inv));
-            acc = fadd(acc, fmul(a.x, v.x));
-            acc = fadd(acc, fmul(a.y, v.y));
-            acc = fadd(acc, fmul(a.z, v.z));
-            acc = fadd(acc, fmul(a.w, v.w));
+                for (int j = 0; j < EX_COLS; j += 4) {
+                    const float4 p = *reinterpret_cast<const float4*>(w + j), u = *reinterpret_cast<const float4*>(x + j);
+                    acc = fadd(acc, fmul(p.x, u.x));
+                    acc = fadd(acc, fmul(p.y, u.y));
+                    acc = fadd(acc, fmul(p.z, u.z));
+                    acc = fadd(acc, fmul(p.w, u.w));
+                }
+            }
+            __syncthreads();
         }
-        out[e] = bias && e < E ? fadd(acc, bias[e]) : acc;
+        if (r < nr)
+            a.exact[(int64_t)s_tok[i] * rows + e0 + r] = a.bias && e0 + r < a.E ? fadd(acc, a.bias[e0 + r]) : acc;
     }
-    __syncthreads();
 }
 
 struct FewRouting {  // in shared memory: [T][k], [T][k], [T]
@@ -779,7 +831,8 @@ __global__ __launch_bounds__(FE_T, 1) void k_few_experts(const __grid_constant__
     __shared__ int s_idx[FEW_T * 32], s_use[FE_ITEMS], s_mask[FE_T], s_item[FE_ITEMS], s_count[FE_W], s_nuse, s_ok;
     __shared__ ApartInputs s_apart;
     __shared__ uint32_t s_open, s_hblk[2][FE_SLOTS + 1];
-    __shared__ float s_gate[FEW_T * 32], s_share[FEW_T], s_inv, s_part[FE_PART * 8];
+    __shared__ __align__(16) float s_part[FE_PART * 8];
+    __shared__ float s_gate[FEW_T * 32], s_share[FEW_T];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     constexpr int d = 1024 * CPL, nb = d / 32, f = 128 * BPQ;
     const int T = a.T, E = a.E, k = a.k, slots = k + a.has_shared;
@@ -803,14 +856,15 @@ __global__ __launch_bounds__(FE_T, 1) void k_few_experts(const __grid_constant__
         lane == 0)
         atomicOr(&s_open, 1u << warp);
     __syncthreads();
-    for (uint32_t open = s_open; open; open &= open - 1) {
-        // s_part: the token's logits, then the scratch of its top-k
-        const int t = __ffs(open) - 1;
-        exact_logits(a.x + (int64_t)t * d, a.router, a.bias, d, E, a.norm, s_part, &s_inv);
-        if (warp == 0)
-            topk_token<NPL, true>(s_part, 0, E, k, a.has_shgate, s_idx + t * k, s_gate + t * k, s_share + t, nullptr,
-                                  s_part + FE_MAXE, s_item, lane);
-        __syncthreads();
+    if (const uint32_t open = s_open) {  // the same in every CTA
+        exact_logits(a, open, s_part);
+        if (!grid_barrier(a.bar + 1, a.err, &s_ok)) return;
+        for (int half = 0; half < 2; ++half) {  // s_part: the scratch of eight tokens' top-k
+            if (warp / 8 == half && (open >> warp) & 1)
+                topk_token<NPL>(a.exact, warp, E, k, a.has_shgate, s_idx, s_gate, s_share, nullptr,
+                                s_part + warp % 8 * FE_T, s_item + 32 * warp, lane);
+            __syncthreads();
+        }
     }
     // The group's work: items of an expert and up to four of its tokens, which share the decoded
     // weights. The shared expert's come first, then those of several tokens, so that the
@@ -952,7 +1006,7 @@ __global__ __launch_bounds__(FE_T, 1) void k_few_experts(const __grid_constant__
 constexpr size_t FEW_X_BYTES = 180 * 1024;  // inputs of the tokens a CTA keeps for gate/up
 
 struct FewBufs {
-    float *logits, *eps, *h;
+    float *logits, *eps, *exact, *h;
     uint32_t *xfix, *bar;
     float* xap;
     size_t bytes;
@@ -960,9 +1014,10 @@ struct FewBufs {
 FewBufs few_carve(const pi_moe_layer* L, int64_t T, char* base) {
     PiBump b{base};
     FewBufs o;
-    o.bar = b.take<uint32_t>(1);
+    o.bar = b.take<uint32_t>(2);
     o.logits = b.take<float>(T * (L->E + 1));
     o.eps = b.take<float>(T * (L->E + 1));
+    o.exact = b.take<float>(T * (L->E + 1));
     o.xfix = b.take<uint32_t>(T * (L->d / 32) * FX_WORDS);
     o.xap = b.take<float>(T * L->d);
     o.h = b.take<float>(T * (L->k + (L->has_shared ? 1 : 0)) * L->f);
@@ -1058,6 +1113,7 @@ int few_forward(pi_ctx* ctx, const pi_moe_layer* L, const float* x, int64_t T, f
     a.xap = B.xap;
     a.logits = B.logits;
     a.eps = B.eps;
+    a.exact = B.exact;
     a.router = L->router;
     a.bias = L->bias;
     a.norm = norm ? 1 : 0;

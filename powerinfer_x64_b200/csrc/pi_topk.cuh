@@ -6,9 +6,8 @@
 // largest key with redux.sync max (keys: probability bits + 2, order-preserving
 // for non-negative floats; 1 for NaN, 0 for taken) and then the lowest index
 // holding it with redux.sync min.
-// logits: in global memory (read past L1: other CTAs may have written them), or with SHARED
-// in shared memory.
-template <int NPL, bool SHARED = false>
+// The logits are read past L1: other CTAs may have written them.
+template <int NPL>
 PI_DEV void topk_token(const float* __restrict__ logits, int t, int E, int k, int has_shgate,
                        int32_t* __restrict__ idx, float* __restrict__ gates, float* __restrict__ shscale,
                        int32_t* __restrict__ counts, float* p, int* sel, int lane) {
@@ -18,7 +17,7 @@ PI_DEV void topk_token(const float* __restrict__ logits, int t, int E, int k, in
 #pragma unroll
     for (int j = 0; j < NPL; ++j) {
         const int e = lane + 32 * j;
-        l[j] = (e < E) ? (SHARED ? lr[e] : __ldcg(lr + e)) : -INFINITY;
+        l[j] = (e < E) ? __ldcg(lr + e) : -INFINITY;
         if (e < E) m = fmaxf(m, l[j]);
     }
 #pragma unroll
@@ -86,6 +85,6 @@ PI_DEV void topk_token(const float* __restrict__ logits, int t, int E, int k, in
         gates[(size_t)t * k + lane] = (ssum > 0.0f) ? fdiv(pe, ssum) : pe;
         if (counts) atomicAdd(&counts[e], 1);
     }
-    if (lane == 0 && shscale) shscale[t] = has_shgate ? sigmoid_ref(SHARED ? lr[E] : __ldcg(lr + E)) : 1.0f;
+    if (lane == 0 && shscale) shscale[t] = has_shgate ? sigmoid_ref(__ldcg(lr + E)) : 1.0f;
     __syncwarp();
 }
