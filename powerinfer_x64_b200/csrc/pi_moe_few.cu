@@ -254,10 +254,13 @@ __global__ __launch_bounds__(FL_T) void k_few_logits(const FewLogitArgs a) {
         const float l = __shfl_sync(0xffffffffu, upto, 31);
         if (lane == 0) {
             const float b = a.bias && e < a.E ? a.bias[e] : 0.0f;
-            float bound = 2.2f * B + 12.0f * A + 4.0f * (fabsf(l) + fabsf(b));
+            float bound = 2.2f * B + 12.0f * A + 4.0f * fabsf(l);
             if (a.norm) bound += ((float)d * 0.125f + 64.0f) * fabsf(l);
+            // exact: nothing but zeros to add (products that vanish here and, other norms, not in the
+            // reference are below 2^-148 and move no probability), or a masked expert
+            const bool exact = A == 0.0f || (b == -INFINITY && bound < INFINITY);
             a.logits[(int64_t)(t0 + t) * (a.E + 1) + e] = l + b;
-            a.eps[(int64_t)(t0 + t) * (a.E + 1) + e] = bound * 5.9604645e-8f;
+            a.eps[(int64_t)(t0 + t) * (a.E + 1) + e] = exact ? 0.0f : (bound + 4.0f * fabsf(b)) * 5.9604645e-8f;
         }
     }
 }
@@ -580,7 +583,10 @@ PI_DEV bool grid_barrier(uint32_t* bar, uint32_t* err, int* s_ok) {
 // Top-k and gates of one token from logits and their bounds, by one warp; false where the
 // bounds leave the reference's choice open. The reference ranks rounded probabilities
 // (model/mod.rs:1278-1303): logits apart by 2^-16 (1 + their distance from the largest) have
-// distinct ones as long as none underflows, hence the second and third conditions. Gates are
+// distinct ones as long as none underflows. So the choice is certain where the selected stand
+// that far above the others; or where some of both tie exactly (a row of zeros, which pads a
+// batch), the lowest indexes among those being the selected ones, and the rest stand that far
+// above or below them. A logit of -inf with a bound of 0 is a masked expert. Gates are
 // renormalised over the selected, so the softmax's full sum cancels.
 template <int NPL>
 PI_DEV bool topk_certain(const float* logits, const float* eps, int E, int k, int has_shgate, int32_t* idx,
@@ -588,22 +594,22 @@ PI_DEV bool topk_certain(const float* logits, const float* eps, int E, int k, in
     float l[NPL], hi[NPL];
     uint32_t key[NPL];
     float m = -INFINITY;
-    bool finite = true;
+    bool known = true;
 #pragma unroll
     for (int j = 0; j < NPL; ++j) {
         const int e = lane + 32 * j;
         l[j] = e < E ? __ldcg(logits + e) : -INFINITY;
         const float ep = e < E ? __ldcg(eps + e) : 0.0f;
-        hi[j] = l[j] + ep;
-        if (e < E) finite = finite && fabsf(l[j]) < INFINITY && ep < INFINITY;
-        const uint32_t b = __float_as_uint(l[j]);
+        hi[j] = l[j] + ep;  // l itself where the bound is 0, above it otherwise
+        known = known && ((fabsf(l[j]) < INFINITY && ep < INFINITY) || (l[j] == -INFINITY && ep == 0.0f));
+        const uint32_t b = __float_as_uint(l[j] + 0.0f);  // -0 as 0
         key[j] = e < E ? ((b & 0x80000000u) ? ~b : (b | 0x80000000u)) : 0u;
         m = fmaxf(m, l[j]);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (!__all_sync(0xffffffffu, finite)) return false;
-    int mine = 0x7fffffff;      // lane r: the r-th selected expert, its logit
+    if (!__all_sync(0xffffffffu, known)) return false;
+    int mine = 0x7fffffff;  // lane r: the r-th selected expert, its logit and that one's lower end
     float lm = 0.0f, low = INFINITY;
     for (int r = 0; r < k; ++r) {
         uint32_t mk = 0;
@@ -621,22 +627,38 @@ PI_DEV bool topk_certain(const float* logits, const float* eps, int E, int k, in
             for (int j = 0; j < NPL; ++j)
                 if (j == (e >> 5)) {
                     key[j] = 0;
-                    lo = 2.0f * l[j] - hi[j];
+                    lo = l[j] > -INFINITY ? 2.0f * l[j] - hi[j] : -INFINITY;
                     hi[j] = -INFINITY;
                 }
         }
-        low = fminf(low, __shfl_sync(0xffffffffu, lo, e & 31));
+        lo = __shfl_sync(0xffffffffu, lo, e & 31);
         if (lane == r) {
             mine = e;
             lm = __uint_as_float((mk & 0x80000000u) ? (mk ^ 0x80000000u) : ~mk);
+            low = lo;
         }
     }
-    float high = -INFINITY;  // upper end of those not selected
+    const float v = __shfl_sync(0xffffffffu, lm, k - 1);  // the last selected
+    bool tie = false;
+    float high = -INFINITY;  // upper end of those not selected, but for those that tie with v
 #pragma unroll
-    for (int j = 0; j < NPL; ++j) high = fmaxf(high, lane + 32 * j < E ? hi[j] : -INFINITY);
+    for (int j = 0; j < NPL; ++j) {
+        const bool same = hi[j] == v && l[j] == v;
+        tie = tie || same;
+        high = fmaxf(high, same ? -INFINITY : hi[j]);
+    }
+    tie = __any_sync(0xffffffffu, tie) && __shfl_sync(0xffffffffu, low, k - 1) == v;
+    if (!tie)
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
-    if (!(low - m > -80.0f) || !(low > high + 0x1p-16f * (1.0f + (m - low)))) return false;
+        for (int j = 0; j < NPL; ++j) high = fmaxf(high, hi[j]);
+    if (tie && low == v && lm == v) low = INFINITY;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+        low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+    }
+    const float edge = tie ? v : low, apart = 0x1p-16f * (1.0f + (m - edge));
+    if (!(edge - m > -80.0f) || !(edge > high + apart) || (tie && !(low > v + apart))) return false;
     const float p = lane < k ? expf(lm - m) : 0.0f, sum = warp_sum(p);
     int rank = 0;  // ascending experts, model/mod.rs:1303
     for (int r = 0; r < k; ++r) rank += __shfl_sync(0xffffffffu, mine, r) < mine;

@@ -130,3 +130,87 @@ def test_open_tokens_cost_one_more_step(orc, norm):
     tied = _make(w, d, f, E, k)
     base, open_ = (_device_us(lambda: L.forward(x, rmsnorm=norm, path="fused")) for L in (plain, tied))
     assert open_ < 2.5 * base, (open_, base)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("bias", [None, "steps", "masks", "few", "all", "mixed"])
+def test_rows_of_zeros_and_masked_experts(orc, norm, bias):
+    """A batch padded with zeros (every logit is its bias: they tie, or tie in steps), experts that a bias of
+    -inf takes out, so that enough, fewer than k or none are left, and router rows of zeros."""
+    import torch
+
+    d, f, E, k = 1024, 128, 40, 6
+    rng = np.random.default_rng(31)
+    w = _layer(orc, rng, d, f, E, k, "gated", False)
+    w["router"].reshape(E, d)[[3, 8, 30]] = 0.0
+    b = np.zeros(E, np.float32)
+    if bias == "steps":
+        b[:] = rng.integers(0, 4, E)
+    elif bias == "masks":
+        b[rng.permutation(E)[:20]] = -np.inf
+    elif bias == "few":
+        b[rng.permutation(E)[: E - k + 2]] = -np.inf
+    elif bias == "mixed":
+        b[:] = rng.choice(np.float32([-np.inf, -0.0, 0.0, 1.0, 3e-4, -100.0, 2.0 ** -17]), E)
+    elif bias == "all":
+        b[:] = -np.inf
+    w["bias"] = None if bias is None else b
+    x = rng.standard_normal((16, d)).astype(np.float32)
+    x[5:] = 0.0
+    x[7, 3] = 1e-30
+    L = _make(w, d, f, E, k)
+    xd = torch.from_numpy(x).cuda()
+    y = L.forward(xd, rmsnorm=norm, residual=True, path="fused")
+    L.ctx.sync_check()
+    if bias == "all":  # no probability anywhere: NaN, as the layer's other path gives
+        want = L.forward(xd, rmsnorm=norm, residual=True, path="gemv")
+        assert torch.equal(torch.isnan(y), torch.isnan(want))
+        return
+    # an f32 operation that underflows is off by 2^-150 at most, whatever its value: fewer than 2^25 of
+    # them lead to an output, and what follows them multiplies by less than 2^5
+    want, tol = _reference(orc, w, x, d, f, E, k, norm, True)
+    _close(y, want, tol + 2.0 ** -120)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bias", [None, "steps", "mixed"])
+def test_exact_ties_among_other_logits(orc, bias):
+    """Router rows of zeros: their logits tie, exactly and at any place among the others, and which of them
+    are chosen shows in the output."""
+    import torch
+
+    d, f, E, k, T = 1024, 128, 300, 9, 16
+    rng = np.random.default_rng(33)
+    w = _layer(orc, rng, d, f, E, k, None, False)
+    w["router"].reshape(E, d)[rng.permutation(E)[: E - 12]] = 0.0
+    if bias:
+        w["bias"] = rng.choice(np.float32([0.0, 0.5, -0.25]) if bias == "steps" else
+                               np.float32([-np.inf, -0.0, 0.0, 1e-6, 2.0 ** -17]), E)
+    x = rng.standard_normal((T, d)).astype(np.float32)
+    L = _make(w, d, f, E, k)
+    y = L.forward(torch.from_numpy(x).cuda(), path="fused")
+    L.ctx.sync_check()
+    _close(y, *_reference(orc, w, x, d, f, E, k, False, False))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", ["zeros", "masks"])
+def test_padding_and_masks_are_certain(orc, what):
+    """Neither a row of zeros nor a masked expert leaves a choice open: the time is that of other tokens."""
+    import torch
+
+    d, f, E, k = 2048, 128, 64, 4
+    rng = np.random.default_rng(32)
+    w = _layer(orc, rng, d, f, E, k, None, False)
+    plain = _make(w, d, f, E, k)
+    w["bias"] = np.zeros(E, np.float32)
+    x = torch.from_numpy(rng.standard_normal((16, d)).astype(np.float32)).cuda()
+    base = _device_us(lambda: plain.forward(x, rmsnorm=True, path="fused"))
+    if what == "zeros":
+        x[1:] = 0.0
+    else:
+        w["bias"][::5] = -np.inf
+    L = _make(w, d, f, E, k)
+    other = _device_us(lambda: L.forward(x, rmsnorm=True, path="fused"))
+    assert other < 1.2 * base + 2.0, (other, base)
