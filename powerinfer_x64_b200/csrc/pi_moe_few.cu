@@ -555,16 +555,17 @@ __device__ __noinline__ void apart_down(const FewExpertArgs& a, const int* idx, 
     __syncthreads();
 }
 
-// Barrier of a cooperatively launched grid, each used once: *bar counts up from 0. The wait is
-// bounded (2^24 polls, the later ones 32 ns apart: about half a second); when it runs out
-// the kernel records PI_DEVERR_TIMEOUT and the CTA returns.
+// Barrier of a cooperatively launched grid, each used once: *bar counts up from 0. The wait
+// ends after 2^31 cycles of the SM (1.1 s at 1.965 GHz), whatever a poll takes: the kernel then
+// records PI_DEVERR_TIMEOUT and the CTA returns.
 PI_DEV bool grid_barrier(uint32_t* bar, uint32_t* err, int* s_ok) {
     __syncthreads();
     if (threadIdx.x == 0) {
         __threadfence();
         atomicAdd(bar, 1u);
         int ok = 0;
-        for (uint32_t it = 0; it < (1u << 24); ++it) {
+        long long start = 0;
+        for (uint32_t it = 0;; ++it) {
             uint32_t v;
             asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(bar) : "memory");
             if (v >= gridDim.x) {
@@ -572,6 +573,11 @@ PI_DEV bool grid_barrier(uint32_t* bar, uint32_t* err, int* s_ok) {
                 break;
             }
             if (it > 4096) __nanosleep(32);
+            if ((it & 255) == 255) {
+                const long long now = clock64();
+                if (it == 255) start = now;
+                else if (now - start > (1ll << 31)) break;
+            }
         }
         if (!ok) atomicOr(err, PI_DEVERR_TIMEOUT);
         *s_ok = ok;
