@@ -214,3 +214,19 @@ def test_padding_and_masks_are_certain(orc, what):
     L = _make(w, d, f, E, k)
     other = _device_us(lambda: L.forward(x, rmsnorm=True, path="fused"))
     assert other < 1.2 * base + 2.0, (other, base)
+
+
+@pytest.mark.gpu
+def test_a_token_more_than_fits_one_group(orc):
+    """4096 wide, the inputs of 12 tokens fit a CTA; thirteen are worked on as seven and six, at hardly more than
+    the price of twelve."""
+    import torch
+
+    d, f, E, k = 4096, 256, 32, 4
+    rng = np.random.default_rng(41)
+    w = _layer(orc, rng, d, f, E, k, None, False)
+    w["bias"] = np.linspace(0.0, 30.0, E).astype(np.float32)[rng.permutation(E)]  # no choice is open
+    L = _make(w, d, f, E, k)
+    x = torch.from_numpy(rng.standard_normal((13, d)).astype(np.float32)).cuda()
+    fits, more = (_device_us(lambda: L.forward(x[:T], path="fused")) for T in (12, 13))
+    assert more < 1.2 * fits, (more, fits)
