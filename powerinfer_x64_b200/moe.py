@@ -27,6 +27,13 @@ def _torch():
     return torch
 
 
+def _path_flags(path: str) -> int:
+    try:
+        return {"auto": 0, "gemv": PI_FWD_FORCE_GEMV, "gemm": PI_FWD_FORCE_GEMM}[path]
+    except KeyError:
+        raise PiError(PI_ERR_ARG, f"moe: no path {path!r} in this call") from None
+
+
 class MoeLayer:
     """Device-resident MoE FFN layer built from GGUF-layout tensors.
 
@@ -121,7 +128,7 @@ class MoeLayer:
         if T == 0:
             return out
         flags = (PI_FWD_RMSNORM if rmsnorm else 0) | (PI_FWD_RESIDUAL if residual else 0)
-        flags |= {"auto": 0, "gemv": PI_FWD_FORCE_GEMV, "gemm": PI_FWD_FORCE_GEMM}[path]
+        flags |= _path_flags(path)
         flags |= PI_FWD_FAST_SUM if fast else 0
         self.ctx.check(lib().pi_moe_forward(self.ctx.h, self.h, ptr(xd), T, ptr(out), flags, stream_ptr()))
         return out
@@ -172,7 +179,8 @@ class MoeLayer:
                        path: str = "auto", fast: bool = False):
         """``forward`` that also returns the routing it used: (out, dict(idx, gates,
         counts, offsets, perm)) as ``route`` returns them, computed on the
-        (optionally RMS-normed) tokens the forward itself routed."""
+        (optionally RMS-normed) tokens the forward itself routed. path: "auto", "gemv" or "gemm"
+        (the fused path does not give its routing out)."""
         if stream is not None:
             return self._on_stream(stream, self.forward_routed, x, out, rmsnorm=rmsnorm, residual=residual,
                                    path=path, fast=fast)
@@ -190,7 +198,7 @@ class MoeLayer:
         if T == 0:
             return out, o
         flags = (PI_FWD_RMSNORM if rmsnorm else 0) | (PI_FWD_RESIDUAL if residual else 0)
-        flags |= {"auto": 0, "gemv": PI_FWD_FORCE_GEMV, "gemm": PI_FWD_FORCE_GEMM}[path]
+        flags |= _path_flags(path)
         flags |= PI_FWD_FAST_SUM if fast else 0
         self.ctx.check(lib().pi_moe_forward_routed(self.ctx.h, self.h, ptr(xd), T, ptr(out), flags, ptr(o["idx"]),
                                                    ptr(o["gates"]), ptr(o["counts"]), ptr(o["offsets"]),
