@@ -17,7 +17,6 @@ import numpy as np
 
 from . import quant
 from ._lib import Context, lib, ptr, stream_ptr
-from .logprobs import token_logprobs
 
 
 def lm_head_slices(n_out: int, n_gpus: int):
@@ -90,6 +89,8 @@ class LmHead:
     def logprobs(self, x, targets=None, n_top: int = 0):
         """``token_logprobs`` of the full logits of x [T, n_in]: log probabilities of the
         given tokens, entropy and the n_top best alternatives."""
+        from .logprobs import token_logprobs
+
         return token_logprobs(self.forward(x), targets=targets, n_top=n_top)
 
 
