@@ -37,13 +37,14 @@ class AdapterBank:
         for v, dt, what in ((ranks, torch.int32, "ranks int32"), (scales, torch.float32, "scales f32")):
             if v is not None and (v.dtype != dt or v.shape != (n,) or v.device != a.device):
                 raise PiError(PI_ERR_ARG, f"adapters: {what} [n] on the adapters' device")
+        a, b = a.detach(), b.detach()  # copies of parameters; set() writes into them
         self.n, self.rank, self.n_in, self.n_out, self.device = n, R, n_in, b.shape[1], a.device
         pad = -R % 8
         self.a = torch.nn.functional.pad(a, (0, 0, 0, pad)) if pad else a.clone(memory_format=torch.contiguous_format)
         self.b = torch.nn.functional.pad(b, (0, pad)) if pad else b.clone(memory_format=torch.contiguous_format)
         full = torch.full((n,), R, dtype=torch.int32, device=a.device)
         self.ranks = full if ranks is None else torch.minimum(ranks, full)
-        self.scales = torch.ones(n, dtype=torch.float32, device=a.device) if scales is None else scales.clone()
+        self.scales = torch.ones(n, dtype=torch.float32, device=a.device) if scales is None else scales.detach().clone()
         self.desc = PiLoraBank(self.a.data_ptr(), self.b.data_ptr(), self.ranks.data_ptr(), self.scales.data_ptr(),
                                _DTYPES[a.dtype], n, R + pad)
         self._desc = C.byref(self.desc)
@@ -55,8 +56,8 @@ class AdapterBank:
         r = a.shape[0] if a.dim() == 2 else -1
         if not 0 <= r <= self.rank or tuple(a.shape) != (r, self.n_in) or tuple(b.shape) != (self.n_out, r):
             raise PiError(PI_ERR_ARG, f"adapters: need a [r, {self.n_in}] and b [{self.n_out}, r], r <= {self.rank}")
-        self.a[i, :r].copy_(a)
-        self.b[i, :, :r].copy_(b)
+        self.a[i, :r].copy_(a.detach())
+        self.b[i, :, :r].copy_(b.detach())
         self.ranks[i] = r
         self.scales[i] = scale
 
