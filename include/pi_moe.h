@@ -207,7 +207,7 @@ int pi_moe_forward_routed(pi_ctx* ctx, pi_moe_layer* layer, const float* x, int6
  * row) is kept in f32 or within 2^-22 of one that four of its block reach a 32nd of, so
  * within 2^-17 of the block's fourth largest magnitude; NaN and infinities act as in f32.
  * flags: PI_FWD_RMSNORM | PI_FWD_RESIDUAL. x and out 16-byte aligned; out
- * may be x. workspace: pi_moe_fused_workspace(layer, T) bytes, 256-byte aligned, that
+ * may be x, but not overlap it otherwise. workspace: pi_moe_fused_workspace(layer, T) bytes, 256-byte aligned, that
  * nothing else uses until the call's work is done (two captured graphs need one each);
  * NULL: the stream's scratch arena (pi_ctx_reserve before a capture). The second kernel
  * is a cooperative launch of one CTA per SM, so such calls on several streams take turns. */

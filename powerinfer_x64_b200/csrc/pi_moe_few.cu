@@ -1096,6 +1096,8 @@ int few_forward(pi_ctx* ctx, const pi_moe_layer* L, const float* x, int64_t T, f
     if (!x || !out) return pi_set_error(ctx, PI_ERR_ARG, "moe fused: null pointer");
     if ((((uintptr_t)x | (uintptr_t)out) & 15) || ((uintptr_t)workspace & 255))
         return pi_set_error(ctx, PI_ERR_ARG, "moe fused: x and out 16-byte, the workspace 256-byte aligned");
+    if (x != out && x < out + T * L->d && out < x + T * L->d)  // a row would be written before another CTA reads it
+        return pi_set_error(ctx, PI_ERR_ARG, "moe fused: out may be x, but not overlap it otherwise");
     const size_t need = few_carve(L, T, nullptr).bytes;
     if (workspace && workspace_bytes < need) return pi_set_error(ctx, PI_ERR_SHORT, "moe fused: workspace too small");
     PiDeviceGuard dev(ctx->device);
