@@ -163,7 +163,8 @@ PI_DEV float fix_value(const int (&s)[3]) { return fmaf((float)s[0], 65536.0f, (
 // below d u < 2.5e-4 of that. So |reference - here| <= u (2.2 B + 12 A + 4 (|l| + |bias|)), A =
 // sum |p|, which leaves 3 u A for the normed inputs' own roundings. RMSNorm itself scales
 // all inputs of a token alike: the reference's sum of squares, d / 4 sequential additions
-// in four lanes, moves a logit by at most (d / 8 + 64) u |l|, added with the bias in mind.
+// in four lanes, moves a logit by at most (d / 8 + 4) u |l|, this one's, d / 32 fused steps and a
+// join of five, by (d / 64 + 5) u |l|: 72 u and d / 8 u at n_embd 4096, held as 96.
 // ---------------------------------------------------------------------------
 constexpr int FL_T = 256, FL_W = FL_T / 32;
 constexpr int FL_GROUP = 4;               // tokens of a CTA
@@ -255,7 +256,7 @@ __global__ __launch_bounds__(FL_T) void k_few_logits(const FewLogitArgs a) {
         if (lane == 0) {
             const float b = a.bias && e < a.E ? a.bias[e] : 0.0f;
             float bound = 2.2f * B + 12.0f * A + 4.0f * fabsf(l);
-            if (a.norm) bound += ((float)d * 0.125f + 64.0f) * fabsf(l);
+            if (a.norm) bound += ((float)d * 0.125f + 96.0f) * fabsf(l);
             // exact: nothing but zeros to add (products that vanish here and, other norms, not in the
             // reference are below 2^-148 and move no probability), or a masked expert
             const bool exact = A == 0.0f || (b == -INFINITY && bound < INFINITY);
