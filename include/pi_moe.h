@@ -370,6 +370,7 @@ typedef struct pi_lora_bank {
  * exact integer dot times d_w d_x with one fused multiply-add, so results equal
  * pi_matvec_col_major's to f32 rounding, not bit for bit. Q4_0 weights use f32 x (in
  * two f16 terms, within 2^-22 of each value); a token with a NaN or infinity gives NaN.
+ * An infinity in the used part of an adapter gives NaN or infinities in its tokens' rows.
  * workspace: pi_proj_workspace(proj, T, bank) bytes, 256-byte aligned, that nothing
  * else uses until the call's work is done (two captured graphs need one each). NULL:
  * the stream's scratch arena (pi_ctx_reserve before a capture). */

@@ -58,6 +58,8 @@ struct LpStat {
     float m, s, w;
 };
 
+// 2^a within 2 units in the last place (the special-function unit's; 2^-22 of each term, as much as
+// the rounding of its argument). expf would take the kernel's issue slots, its bound for many rows.
 PI_DEV float ex2(float a) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a));

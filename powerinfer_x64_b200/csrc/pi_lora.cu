@@ -544,7 +544,8 @@ __global__ __launch_bounds__(GEMM_T, 2) void k_proj_gemm(const ProjArgs p) {
 // ---------------------------------------------------------------------------
 // k_proj_adapters: y_t += B_a h_t. In a chunk of 64 tokens those of one adapter, up to eight
 // together, are the columns of a product on the tensor cores (B exact in tf32 for f16 and
-// bf16, two tf32 terms for f32; h in two terms); a warp's step is two tiles of 16 rows of one
+// bf16, two tf32 terms for f32; h in two terms: what the second terms leave, and the product of two
+// second terms, is below 2^-21 of each product, as a few f32 roundings are); a warp's step is two tiles of 16 rows of one
 // such group. A token is in one group only, so an adapter's NaN stays with its requests and
 // every sum has one owner.
 //
