@@ -360,13 +360,14 @@ PI_DEV void chunk_products(const RowChunk& k, const uint32_t* const (&xs)[TB], i
 }
 
 // Which inputs of a group's tokens are held apart: a bit for each block that has some, and where they
-// are few the list of them in order, each with its value in every token (0 where it is not held
-// apart). Outliers mostly stand at the same few places in every token.
+// are few the list of them, by their place modulo 8 and then in order, each with its value in every
+// token (0 where it is not held apart). Outliers mostly stand at the same few places in every token.
 constexpr int AP_LIST = 64;
 struct ApartInputs {
     uint32_t any, n;  // n > AP_LIST: too many for the list
     uint32_t blk[FEW_T][4];
-    uint16_t at[AP_LIST];
+    uint16_t found[AP_LIST], at[AP_LIST];  // in order; by place modulo 8, whose parts start at first[]
+    int first[9];
     float value[FEW_T][AP_LIST];
 };
 
@@ -386,10 +387,18 @@ __device__ __noinline__ void list_apart(ApartInputs& s, const uint32_t* s_x, con
                 if (tid >= o) upto += v;
             }
             for (int i = n + upto - __popc(m); m; m &= m - 1, ++i)
-                if (i < AP_LIST) s.at[i] = (uint16_t)((tid + 32 * c) * 32 + __ffs(m) - 1);
+                if (i < AP_LIST) s.found[i] = (uint16_t)((tid + 32 * c) * 32 + __ffs(m) - 1);
             n += __shfl_sync(0xffffffffu, upto, 31);
         }
         if (tid == 0) s.n = n;
+        __syncwarp();
+        if (tid < 9 && n <= AP_LIST) {
+            int pos = 0;
+            for (int i = 0; i < n; ++i) pos += (s.found[i] & 7) < tid;
+            s.first[tid] = pos;
+            for (int i = 0; i < n; ++i)
+                if ((s.found[i] & 7) == tid) s.at[pos++] = s.found[i];
+        }
     }
     __syncthreads();
     if (s.n <= AP_LIST)
@@ -405,8 +414,8 @@ __device__ __noinline__ void list_apart(ApartInputs& s, const uint32_t* s_x, con
 
 // c[t] += this lane's part of what the values held apart add to row-vector lane / 8 of an item's unit
 // (rows row, row + 1 of expert e) for its tokens, numbered in the bytes of toks within the CTA's
-// group: every eighth of the list, or of the elements of the blocks that have some. The weights,
-// read a moment ago, come from L2. A function of its own: it is rare, and the loop around it has
+// group: of all elements those at lane % 8 modulo 8, in order, whichever tokens stand beside one another (so
+// a token's sums are the same alone). The weights, read a moment ago, come from L2. A function of its own: it is rare, and the loop around it has
 // no registers to spare.
 template <int CPL>
 __device__ __noinline__ float4 apart_products(const FewExpertArgs& a, const ApartInputs& s, const uint32_t* s_x, int t0,
@@ -420,7 +429,7 @@ __device__ __noinline__ float4 apart_products(const FewExpertArgs& a, const Apar
     float sum[FE_TB] = {c.x, c.y, c.z, c.w};
     if (s.n <= AP_LIST) {
 #pragma unroll 2
-        for (int q = lane & 7; q < s.n; q += 8) {
+        for (int q = s.first[lane & 7]; q < s.first[(lane & 7) + 1]; ++q) {
             const int at = s.at[q];
             const float v = nib_value(w + (at >> 5) * 16, at & 31, sc[at >> 5]);
 #pragma unroll

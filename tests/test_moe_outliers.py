@@ -140,3 +140,24 @@ def test_an_infinite_hidden_value_acts_as_in_f32(orc):
     assert not torch.isfinite(want[1]).any() and torch.isfinite(want[[0, 2]]).all()
     for test in (torch.isnan, torch.isposinf, torch.isneginf):
         assert torch.equal(test(y), test(want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [5, 40, 300])
+def test_outliers_of_other_tokens_change_nothing(orc, n):
+    """The same bits alone and in a batch whose other tokens have outliers elsewhere, few or more than are
+    listed."""
+    import torch
+
+    d, f, E, k, T = 1024, 128, 6, 2, 16
+    rng = np.random.default_rng(n)
+    L = _make(_layer(orc, rng, d, f, E, k, "gated", False), d, f, E, k)
+    x = rng.standard_normal((T, d)).astype(np.float32)
+    for t in range(T):
+        at = rng.integers(0, d, n)
+        x[t, at] *= 10.0 ** rng.uniform(2.0, 4.0, n)
+    x[3] = rng.standard_normal(d)
+    xd = torch.from_numpy(x).cuda()
+    y = L.forward(xd, path="fused")
+    assert torch.equal(torch.cat([L.forward(xd[t:t + 1], path="fused") for t in range(T)]), y)
+    assert torch.equal(L.forward(xd[4:11], path="fused"), y[4:11])
