@@ -819,11 +819,15 @@ PI_DEV void down_phase(const FewExpertArgs& a, const int d, const FewRouting& r,
         if (t != tok) {
             const float* ht = a.h + (int64_t)t * slots * f;
             turn ^= 1;  // this token's masks; the next one's are cleared meanwhile
-            for (int i0 = 0; i0 < slots * (f / 4); i0 += FE_T) {  // whole warps: eight lanes make a block
-                const int i = min(i0 + tid, slots * (f / 4) - 1), j = i / (f / 4), b = (i & (f / 4 - 1)) >> 3;
-                const uint32_t apart = fix_block(__ldcg(reinterpret_cast<const float4*>(ht) + i),
-                                                 s_h + j * hp + (b / BPQ) * h_quarter(BPQ) + (b % BPQ) * FX_WORDS,
-                                                 i & 7, i0 + tid < slots * (f / 4), nullptr);
+            const int n4 = slots * (f / 4);
+            auto fetch = [&](int i0) { return __ldcg(reinterpret_cast<const float4*>(ht) + min(i0 + tid, n4 - 1)); };
+            float4 v = fetch(0);
+            for (int i0 = 0; i0 < n4; i0 += FE_T) {  // whole warps: eight lanes make a block
+                const int i = min(i0 + tid, n4 - 1), j = i / (f / 4), b = (i & (f / 4 - 1)) >> 3;
+                const float4 now = v;
+                v = fetch(i0 + FE_T);  // on its way meanwhile
+                const uint32_t apart = fix_block(now, s_h + j * hp + (b / BPQ) * h_quarter(BPQ) + (b % BPQ) * FX_WORDS,
+                                                 i & 7, i0 + tid < n4, nullptr);
                 if (apart && (i & 7) == 0) {
                     atomicOr(&s_apart[turn][j], 1u << b);
                     s_apart[turn][FE_SLOTS] = 1;
@@ -1027,7 +1031,7 @@ __global__ __launch_bounds__(FE_T, 1) void k_few_experts(const __grid_constant__
         }
     };
     // two loops: the call takes registers from the one that has it (16 tokens, 256 experts: 78 us, 80 with one).
-    // Four outliers in every token make 78 us 94, a single token's 19.5 us 23.3.
+    // Four outliers in every token make 77 us 95, a single token's 19.6 us 24.2.
     if (!s_apart.any) {
         gate_up(std::false_type());
     } else {
