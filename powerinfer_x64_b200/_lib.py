@@ -201,8 +201,11 @@ def torch_stream(stream, device: int):
     import torch
 
     if hasattr(stream, "cuda_stream"):
+        if stream.device.index != device:
+            raise PiError(PI_ERR_ARG, f"the stream is one of {stream.device}, not of cuda:{device}")
         return stream
-    return torch.cuda.ExternalStream(int(stream), device=device)
+    handle = int(stream)
+    return torch.cuda.ExternalStream(0 if handle == 1 else handle, device=device)  # 1: the default stream's other name
 
 
 def raw_stream(device: int) -> int:

@@ -17,3 +17,16 @@ def test_unknown_paths_are_refused(monkeypatch, call, path):
     with pytest.raises(PiError) as e:
         getattr(L, call)(_Tensor(64, 0), path=path)
     assert e.value.code == PI_ERR_ARG and not lib.calls
+
+
+def test_a_stream_of_another_device_is_refused(monkeypatch):
+    """The work would run on that device's idea of the current stream, in no order with the given one."""
+    import types
+
+    from powerinfer_x64_b200 import PiError, _lib
+
+    there = types.SimpleNamespace(cuda_stream=0x70, device=types.SimpleNamespace(index=1))
+    assert _lib.torch_stream(there, 1) is there
+    with pytest.raises(PiError) as e:
+        _lib.torch_stream(there, 0)
+    assert e.value.code == _lib.PI_ERR_ARG
